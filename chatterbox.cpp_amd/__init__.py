@@ -155,6 +155,64 @@ class T3Cache(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_ctx", ctypes.c_int32)]
 
 
+CBX_KV_F32, CBX_KV_F16 = 0, 1
+
+
+class KvCache(ctypes.Structure):
+    """cbx_kv_cache (include/cbx_kv.h): a pool of key/value pages."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (f, ctypes.c_int32) for f in ("type", "n_layer", "n_pages", "n_head", "page_size")]
+
+
+class KvStreams(ctypes.Structure):
+    """cbx_kv_streams (include/cbx_kv.h): the streams of a pool."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("n_streams", "n_prefix", "max_pages", "n_pages")] + [
+        (f, ctypes.c_void_p) for f in ("tables", "len", "free_pages", "n_free", "parent",
+                                       "prefix_len")]
+
+
+class KvRows(ctypes.Structure):
+    """cbx_kv_rows (include/cbx_kv.h): the rows of one call."""
+
+    _fields_ = [(f, ctypes.c_int32) for f in ("n_rows", "n_tiles", "tile_rows")] + [
+        (f, ctypes.c_void_p) for f in ("stream", "position", "slot", "row_start", "page_start",
+                                       "counts", "tiles", "order")]
+
+
+class KvPlan(ctypes.Structure):
+    """cbx_kv_plan (include/cbx_kv.h): what a call's rows are built from."""
+
+    _fields_ = [
+        ("streams", ctypes.POINTER(KvStreams)),
+        ("rows", ctypes.POINTER(KvRows)),
+        ("page_size", ctypes.c_int32),
+    ] + [(f, ctypes.c_void_p) for f in ("n_new", "state", "release", "len_out", "n_free_out")]
+
+
+class KvAttn(ctypes.Structure):
+    """cbx_kv_attn (include/cbx_kv.h): attention of one layer's rows."""
+
+    _fields_ = [
+        ("cache", ctypes.POINTER(KvCache)),
+        ("streams", ctypes.POINTER(KvStreams)),
+        ("rows", ctypes.POINTER(KvRows)),
+        ("layer", ctypes.c_int32),
+        ("n_head", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("ld_q", ctypes.c_int64),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("ld_kv", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("ld_out", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
 class HeadFile(ctypes.Structure):
     """cbx_head_file (include/cbx_gguf.h): the speech_head of a T3 GGUF."""
 
@@ -266,6 +324,14 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.cbx_t3_prefill.restype = ctypes.c_int
     lib.cbx_t3_prefill.argtypes = [vp, ctypes.POINTER(T3Model), i32, vp, i32, vp, vp, vp,
                                    ctypes.POINTER(T3Cache), vp, vp]
+    lib.cbx_kv_tile_rows.restype = i32
+    lib.cbx_kv_tile_rows.argtypes = [i32, i32]
+    lib.cbx_kv_build.restype = ctypes.c_int
+    lib.cbx_kv_build.argtypes = [vp, ctypes.POINTER(KvPlan), vp]
+    lib.cbx_kv_workspace_bytes.restype = u64
+    lib.cbx_kv_workspace_bytes.argtypes = [ctypes.POINTER(KvAttn)]
+    lib.cbx_kv_attend.restype = ctypes.c_int
+    lib.cbx_kv_attend.argtypes = [vp, ctypes.POINTER(KvAttn), vp]
     lib.cbx_gguf_read_head.restype = ctypes.c_int
     lib.cbx_gguf_read_head.argtypes = [ctypes.c_char_p, ctypes.POINTER(HeadFile)]
     lib.cbx_gguf_load_head.restype = ctypes.c_int
@@ -601,6 +667,175 @@ class Sampler:
         _check(self.lib.cbx_t3_prefill(self.handle, ctypes.byref(model), slots.numel(),
                                        _ptr(slots), k_cache.shape[0], _ptr(tokens), _ptr(inputs),
                                        _ptr(positions), ctypes.byref(c), _ptr(hidden), st))
+
+    # -- paged caches (include/cbx_kv.h) ----------------------------------------
+    @staticmethod
+    def _check_kv(fn, device=None, **tensors):
+        """The C ABI takes raw addresses: shapes (None: any size), dtypes and
+        layout are checked here first, and that all lie on one device."""
+        for name, (t, dt, shape) in tensors.items():
+            if t is None:
+                continue
+            device = t.device if device is None else device
+            if t.dtype != dt or not t.is_contiguous() or t.dim() != len(shape) or \
+                    any(b is not None and a != b for a, b in zip(t.shape, shape)):
+                raise ValueError("%s: %s must be contiguous %s of shape %s, got %s %s%s" % (
+                    fn, name, dt, shape, t.dtype, tuple(t.shape),
+                    "" if t.is_contiguous() else " (not contiguous)"))
+            if t.device != device:
+                raise ValueError("%s: %s is on %s, not %s" % (fn, name, t.device, device))
+        return device
+
+    @staticmethod
+    def kv_cache(k, v):
+        """A cbx_kv_cache over two device tensors, float32 or float16,
+        [n_layer, n_pages, n_kv_head, page_size, 64]."""
+        import torch
+        if k.dtype not in (torch.float32, torch.float16) or k.dim() != 5:
+            raise ValueError("kv_cache: k must be float32 or float16 with 5 dimensions, got %s %s"
+                             % (k.dtype, tuple(k.shape)))
+        shape = tuple(k.shape[:4]) + (64,)
+        Sampler._check_kv("kv_cache", k=(k, k.dtype, shape), v=(v, k.dtype, shape))
+        c = KvCache()
+        c.k, c.v = k.data_ptr(), v.data_ptr()
+        c.type = CBX_KV_F32 if k.dtype == torch.float32 else CBX_KV_F16
+        c.n_layer, c.n_pages, c.n_head, c.page_size = k.shape[:4]
+        c._tensors = (k, v)
+        return c
+
+    @staticmethod
+    def kv_streams(tables, length, free_pages, n_free, *, n_prefix=0, parent=None,
+                   prefix_len=None):
+        """A cbx_kv_streams over device int32 tensors: tables [n_streams,
+        max_pages], length [n_streams], free_pages [n_pages], n_free [1],
+        optional parent and prefix_len [n_streams]."""
+        import torch
+        n, i = tables.shape[0] if tables.dim() else 0, torch.int32
+        if (parent is None) != (prefix_len is None):
+            raise ValueError("kv_streams: parent and prefix_len come together")
+        Sampler._check_kv("kv_streams", tables=(tables, i, (n, None)), length=(length, i, (n,)),
+                          free_pages=(free_pages, i, (None,)), n_free=(n_free, i, (1,)),
+                          parent=(parent, i, (n,)), prefix_len=(prefix_len, i, (n,)))
+        t = KvStreams()
+        t.n_streams, t.max_pages = tables.shape
+        t.n_prefix, t.n_pages = n_prefix, free_pages.numel()
+        t.tables, t.len = tables.data_ptr(), length.data_ptr()
+        t.free_pages, t.n_free = free_pages.data_ptr(), n_free.data_ptr()
+        t.parent = None if parent is None else parent.data_ptr()
+        t.prefix_len = None if prefix_len is None else prefix_len.data_ptr()
+        t._tensors = (tables, length, free_pages, n_free, parent, prefix_len)
+        return t
+
+    @staticmethod
+    def kv_rows(position, slot, row_start, page_start, counts, *, stream=None, tiles=None,
+                order=None, tile_rows=0):
+        """A cbx_kv_rows over device int32 tensors: position, slot (and stream:
+        the prompt form) [n_rows], row_start and page_start [n_streams + 1],
+        counts [4], optional tiles [n_tiles, 4] and, in the step form with
+        tiles, order [n_rows]."""
+        import torch
+        n, i = position.numel(), torch.int32
+        Sampler._check_kv("kv_rows", position=(position, i, (n,)), slot=(slot, i, (n,)),
+                          row_start=(row_start, i, (None,)),
+                          page_start=(page_start, i, (row_start.numel(),)),
+                          counts=(counts, i, (4,)), stream=(stream, i, (n,)),
+                          tiles=(tiles, i, (None, 4)), order=(order, i, (n,)))
+        r = KvRows()
+        r.n_rows, r.tile_rows = n, tile_rows
+        r.n_tiles = 0 if tiles is None else tiles.shape[0]
+        for name, t in (("stream", stream), ("position", position), ("slot", slot),
+                        ("row_start", row_start), ("page_start", page_start), ("counts", counts),
+                        ("tiles", tiles), ("order", order)):
+            setattr(r, name, None if t is None else t.data_ptr())
+        r._tensors = (position, slot, row_start, page_start, counts, stream, tiles, order)
+        return r
+
+    @staticmethod
+    def kv_tile_rows(n_head, n_kv_head):
+        """cbx_kv_tile_rows: rows of a tile."""
+        return load_library().cbx_kv_tile_rows(n_head, n_kv_head)
+
+    @staticmethod
+    def _one_call(fn, streams, rows):
+        n = streams.n_streams
+        if rows._tensors[2].numel() != n + 1:
+            raise ValueError("%s: row_start has %d entries, %d wanted" % (
+                fn, rows._tensors[2].numel(), n + 1))
+        return Sampler._check_kv(fn, streams._tensors[0].device,
+                                 position=(rows._tensors[0], rows._tensors[0].dtype, (rows.n_rows,)))
+
+    @staticmethod
+    def kv_plan(streams, rows, *, page_size, n_new=None, state=None, release=None, len_out=None,
+                n_free_out=None):
+        """A cbx_kv_plan: device int32 tensors n_new, state, release, len_out
+        [n_streams] and n_free_out [1], all optional."""
+        import torch
+        n, i = streams.n_streams, torch.int32
+        dev = Sampler._one_call("kv_plan", streams, rows)
+        Sampler._check_kv("kv_plan", dev, n_new=(n_new, i, (n,)), state=(state, i, (n,)),
+                          release=(release, i, (n,)), len_out=(len_out, i, (n,)),
+                          n_free_out=(n_free_out, i, (1,)))
+        p = KvPlan()
+        p.streams, p.rows = ctypes.pointer(streams), ctypes.pointer(rows)
+        p.page_size = page_size
+        for name, t in (("n_new", n_new), ("state", state), ("release", release),
+                        ("len_out", len_out), ("n_free_out", n_free_out)):
+            setattr(p, name, None if t is None else t.data_ptr())
+        p._tensors = (streams, rows, n_new, state, release, len_out, n_free_out)
+        return p
+
+    def kv_build(self, plan, stream=None):
+        """cbx_kv_build: the plan's page tables, rows and tiles."""
+        st = _stream_ptr() if stream is None else ctypes.c_void_p(stream)
+        _check(self.lib.cbx_kv_build(self.handle, ctypes.byref(plan), st))
+
+    @staticmethod
+    def kv_attn(cache, streams, rows, q, out, *, layer=0, k=None, v=None, scale=0.125,
+                workspace=None):
+        """A cbx_kv_attn: q and out float32 [n_rows, 64 n_head], optional k and
+        v [n_rows, 64 n_kv_head], each with unit stride along its rows (a
+        view of wider rows will do).  Its workspace is allocated here unless
+        given (uint8): two calls that may run at once take a KvAttn each."""
+        import torch
+        dev = Sampler._one_call("kv_attn", streams, rows)
+        if cache._tensors[0].device != dev:
+            raise ValueError("kv_attn: the cache is on another device")
+        n = rows.n_rows
+        for name, t, width in (("q", q, q.shape[-1]), ("out", out, q.shape[-1]),
+                               ("k", k, 64 * cache.n_head), ("v", v, 64 * cache.n_head)):
+            if t is None:
+                continue
+            if t.dtype != torch.float32 or tuple(t.shape) != (n, width) or t.stride(1) != 1 or \
+                    t.device != dev:
+                raise ValueError("kv_attn: %s must be float32 [%d, %d] with unit stride on %s, got "
+                                 "%s %s %s" % (name, n, width, dev, t.dtype, tuple(t.shape),
+                                               t.device))
+        if (k is None) != (v is None) or (k is not None and k.stride(0) != v.stride(0)):
+            raise ValueError("kv_attn: k and v come together, with one row stride")
+        if q.shape[-1] % 64:
+            raise ValueError("kv_attn: q has %d columns, heads have 64" % q.shape[-1])
+        # a single row's stride says nothing
+        ld = lambda t: t.shape[1] if t.shape[0] == 1 else t.stride(0)
+        a = KvAttn()
+        a.cache, a.streams, a.rows = (ctypes.pointer(x) for x in (cache, streams, rows))
+        a.layer, a.n_head, a.scale = layer, q.shape[-1] // 64, scale
+        a.q, a.ld_q, a.out, a.ld_out = q.data_ptr(), ld(q), out.data_ptr(), ld(out)
+        if k is not None:
+            a.k, a.v, a.ld_kv = k.data_ptr(), v.data_ptr(), ld(k)
+        need = load_library().cbx_kv_workspace_bytes(ctypes.byref(a))
+        if workspace is None and need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        if workspace is not None:
+            Sampler._check_kv("kv_attn", dev, workspace=(workspace, torch.uint8, (None,)))
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+        a._tensors = (cache, streams, rows, q, out, k, v, workspace)
+        return a
+
+    def kv_attend(self, attn, stream=None):
+        """cbx_kv_attend: attention of one layer's rows, their new keys and
+        values stored first."""
+        st = _stream_ptr() if stream is None else ctypes.c_void_p(stream)
+        _check(self.lib.cbx_kv_attend(self.handle, ctypes.byref(attn), st))
 
     def decode_step(self, logits, params, tokens, decode, **kw):
         """cbx_decode_step (head=...: cbx_head_decode_step) of one step."""

@@ -635,3 +635,128 @@ int cbx_t3_prefill(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows, const 
 
 
 }  // extern "C"
+
+namespace {
+bool kv_page_ok(int32_t page_size) {
+    return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// What a plan and the calls on its rows have in common.
+int check_kv(const char* fn, const cbx_kv_streams* t, const cbx_kv_rows* r, int32_t page_size) {
+    if (!t || !r) return fail(CBX_ERR_INVALID, "%s: NULL streams or rows", fn);
+    if (!kv_page_ok(page_size))
+        return fail(CBX_ERR_INVALID, "%s: page_size %d (a power of two, 16 .. 256)", fn, page_size);
+    if (t->n_streams < 1 || t->n_streams > cbx::kMaxKvStreams || t->n_prefix < 0 ||
+        t->n_prefix > t->n_streams)
+        return fail(CBX_ERR_INVALID, "%s: n_streams %d outside [1, %d] or n_prefix %d", fn,
+                    t->n_streams, cbx::kMaxKvStreams, t->n_prefix);
+    if (t->max_pages < 1 || (int64_t)t->max_pages * page_size >= 1 << 30 || t->n_pages < 1 ||
+        (int64_t)t->n_pages * page_size > 0x7fffffffLL)
+        return fail(CBX_ERR_INVALID, "%s: max_pages %d, n_pages %d of %d positions", fn, t->max_pages,
+                    t->n_pages, page_size);
+    if (!t->tables || (t->parent && !t->prefix_len))
+        return fail(CBX_ERR_INVALID, "%s: NULL tables, or parent without prefix_len", fn);
+    if (r->n_rows < 1 || (!r->stream && r->n_rows != t->n_streams))
+        return fail(CBX_ERR_INVALID, "%s: n_rows %d (the step form: n_streams)", fn, r->n_rows);
+    if (!r->position || !r->slot || !r->row_start)
+        return fail(CBX_ERR_INVALID, "%s: NULL position, slot or row_start", fn);
+    if (r->tiles) {
+        if (!aligned16(r->tiles) || (!r->stream && !r->order))
+            return fail(CBX_ERR_INVALID, "%s: tiles not 16-byte aligned, or without order", fn);
+        const int64_t want = (int64_t)(r->tile_rows > 0 ? r->n_rows / r->tile_rows : 0) +
+                             (r->stream ? t->n_streams : t->n_prefix);
+        if (r->tile_rows < 1 || r->n_tiles < (want > 1 ? want : 1))
+            return fail(CBX_ERR_INVALID, "%s: %d tiles of %d rows, %lld wanted", fn, r->n_tiles,
+                        r->tile_rows, (long long)want);
+    }
+    return CBX_OK;
+}
+
+int check_kv_attn(const char* fn, const cbx_kv_attn* a) {
+    if (!a || !a->cache) return fail(CBX_ERR_INVALID, "%s: NULL arguments or cache", fn);
+    const cbx_kv_cache& c = *a->cache;
+    const int rc = check_kv(fn, a->streams, a->rows, c.page_size);
+    if (rc != CBX_OK) return rc;
+    if (c.type != CBX_KV_F32 && c.type != CBX_KV_F16)
+        return fail(CBX_ERR_INVALID, "%s: unknown cache type %d", fn, c.type);
+    if (!c.k || !c.v || c.n_layer < 1 || a->layer < 0 || a->layer >= c.n_layer || c.n_head < 1 ||
+        c.n_pages != a->streams->n_pages)
+        return fail(CBX_ERR_INVALID, "%s: cache k/v NULL, layer %d of %d, n_head %d or n_pages %d (%d)",
+                    fn, a->layer, c.n_layer, c.n_head, c.n_pages, a->streams->n_pages);
+    if ((int64_t)c.n_pages * c.page_size * c.n_head >= 0xffffffffLL)
+        return fail(CBX_ERR_UNSUPPORTED, "%s: a layer's pages hold 2^32 or more rows", fn);
+    if (a->n_head < 1 || a->n_head % c.n_head != 0 || a->n_head / c.n_head > 64)
+        return fail(CBX_ERR_UNSUPPORTED, "%s: %d query heads on %d key heads (1 to 64 each)", fn,
+                    a->n_head, c.n_head);
+    if (!a->q || !a->out || (a->k != nullptr) != (a->v != nullptr))
+        return fail(CBX_ERR_INVALID, "%s: NULL q or out, or one of k and v", fn);
+    const int64_t width = (int64_t)64 * a->n_head;
+    if (a->ld_q < width || a->ld_out < width || a->ld_q % 4 || a->ld_out % 4 ||
+        (a->k && (a->ld_kv < (int64_t)64 * c.n_head || a->ld_kv % 4)))
+        return fail(CBX_ERR_INVALID, "%s: row strides %lld, %lld, %lld", fn, (long long)a->ld_q,
+                    (long long)a->ld_out, (long long)a->ld_kv);
+    if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||
+        !aligned16(c.k) || !aligned16(c.v) || !aligned16(a->workspace))
+        return fail(CBX_ERR_INVALID, "%s: an address is not 16-byte aligned", fn);
+    if (a->rows->stream && !a->rows->tiles)
+        return fail(CBX_ERR_INVALID, "%s: the prompt form's tiles are NULL", fn);
+    if (a->rows->tiles && a->rows->tile_rows != cbx_kv_tile_rows(a->n_head, c.n_head))
+        return fail(CBX_ERR_INVALID, "%s: tile_rows %d, %d wanted", fn, a->rows->tile_rows,
+                    cbx_kv_tile_rows(a->n_head, c.n_head));
+    // the launches' grids
+    if ((int64_t)a->rows->n_rows * a->n_head > 0x7fffffffLL ||
+        (a->rows->tiles && (int64_t)a->rows->n_tiles * c.n_head > 0x7fffffffLL))
+        return fail(CBX_ERR_UNSUPPORTED, "%s: %d rows of %d heads", fn, a->rows->n_rows, a->n_head);
+    return CBX_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int32_t cbx_kv_tile_rows(int32_t n_head, int32_t n_kv_head) {
+    if (n_kv_head < 1 || n_head < n_kv_head) return 0;
+    const int32_t group = n_head / n_kv_head;
+    return group < 64 ? 64 / group : 1;
+}
+
+int cbx_kv_build(cbx_sampler* s, const cbx_kv_plan* p, void* stream) {
+    const char* fn = "cbx_kv_build";
+    if (!s || !p) return fail(CBX_ERR_INVALID, "%s: NULL handle or plan", fn);
+    const int rc = check_kv(fn, p->streams, p->rows, p->page_size);
+    if (rc != CBX_OK) return rc;
+    if (!p->streams->len || !p->streams->free_pages || !p->streams->n_free || !p->rows->page_start ||
+        !p->rows->counts)
+        return fail(CBX_ERR_INVALID, "%s: NULL len, free_pages, n_free, page_start or counts", fn);
+    if ((p->len_out != nullptr) != (p->n_free_out != nullptr))
+        return fail(CBX_ERR_INVALID, "%s: one of len_out and n_free_out", fn);
+    DeviceGuard g(s->device);
+    CBX_HIP(cbx::launch_kv_plan(*p, (hipStream_t)stream));
+    return CBX_OK;
+}
+
+uint64_t cbx_kv_workspace_bytes(const cbx_kv_attn* a) {
+    cbx_kv_attn b;
+    if (!a) return 0;
+    b = *a;
+    b.workspace = nullptr;
+    return check_kv_attn("cbx_kv_workspace_bytes", &b) == CBX_OK ? cbx::kv_workspace_bytes(b) : 0;
+}
+
+int cbx_kv_attend(cbx_sampler* s, const cbx_kv_attn* a, void* stream) {
+    const char* fn = "cbx_kv_attend";
+    if (!s) return fail(CBX_ERR_INVALID, "%s: NULL handle", fn);
+    const int rc = check_kv_attn(fn, a);
+    if (rc != CBX_OK) return rc;
+    const uint64_t need = cbx::kv_workspace_bytes(*a);
+    if (need && (!a->workspace || a->workspace_bytes < need))
+        return fail(CBX_ERR_INVALID, "%s: workspace of %llu bytes, %llu wanted", fn,
+                    (unsigned long long)(a->workspace ? a->workspace_bytes : 0),
+                    (unsigned long long)need);
+    DeviceGuard g(s->device);
+    CBX_HIP(cbx::launch_kv_attend(*a, nullptr, nullptr, (hipStream_t)stream));
+    return CBX_OK;
+}
+
+}  // extern "C"

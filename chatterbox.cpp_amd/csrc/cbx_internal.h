@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/cbx_kv.h"
 #include "../../include/cbx_sampler.h"
 #include "../../include/cbx_t3.h"
 
@@ -220,5 +221,15 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
                           const float* inputs, int32_t* positions, const int32_t* state,
                           const int32_t* slots, int32_t n_slots, const cbx_t3_cache& c,
                           float* hidden, void* ws, hipStream_t st);
+
+// The paged cache (cbx_kv_plan.hip, cbx_kv_attn.hip), arguments already checked.
+// kMaxKvStreams: a plan's one workgroup holds 16 streams a thread and, for a
+// step's tiles, two words a stream in LDS.
+// parts set: the output rows go there, split for the next product
+// (cbx_split.h), the scales to inv, instead of to a.out.
+constexpr int32_t kMaxKvStreams = 16384;
+hipError_t launch_kv_plan(const cbx_kv_plan& p, hipStream_t st);
+uint64_t kv_workspace_bytes(const cbx_kv_attn& a);
+hipError_t launch_kv_attend(const cbx_kv_attn& a, uint32_t* parts, float* inv, hipStream_t st);
 
 }  // namespace cbx

@@ -34,6 +34,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "cbx_attn_out.h"
 #include "cbx_group.h"
 #include "cbx_internal.h"
 #include "cbx_split.h"
@@ -294,82 +295,12 @@ struct AttnArgs {
     const int32_t* act;
     const int32_t* slots;  // prefill: the cache slot of each row
     const int32_t* rows;   // prefill: the rows in groups of 16 (t3_group_rows; NULL: in order)
-    float* out;            // [n_rows][n_embd]
-    uint32_t* parts;       // when set, the rows go there instead, split for the
-    float* inv;            //   next product (cbx_split.h), the scales here
+    AttnOut o;             // rows of n_embd
     float scale;           // 1 / sqrt(64)
 };
 
-// Element `lane` (0..63) of head h of row r's attention output, o, from wave
-// 0: to out, or split (the head's 64 values are blocks 2h and 2h + 1 of the
-// row: lanes 0-31 and 32-63, each block scaled by its own largest magnitude,
-// pairs of lanes joining their fp16 halves into dwords).
-__device__ __forceinline__ void attn_store(const AttnArgs& a, int r, int h, int lane, float o) {
-    const int n = a.n_head * kHeadDim;
-    if (!a.parts) {
-        a.out[(int64_t)r * n + h * kHeadDim + lane] = o;
-        return;
-    }
-    float mx = fabsf(o);
-#pragma unroll
-    for (int q = 1; q < 32; q <<= 1) mx = fmaxf(mx, __shfl_xor(mx, q));
-    float sc, sinv;
-    split_scale(mx, sc, sinv);
-    const float y = __fmul_rn(o, sc);
-    const _Float16 hh = (_Float16)y;
-    const _Float16 ll = (_Float16)__fsub_rn(y, (float)hh);
-    const uint32_t hv = __builtin_bit_cast(uint16_t, hh), lv = __builtin_bit_cast(uint16_t, ll);
-    const uint32_t ho = (uint32_t)__shfl_xor((int)hv, 1), lo = (uint32_t)__shfl_xor((int)lv, 1);
-    const int nball = n / 32, kb = 2 * h + (lane >> 5), k = lane & 31;
-    const int T = r >> 4, m = r & 15;
-    if ((lane & 1) == 0) {
-        // dword (k % 8) / 2 of lane 16 (k / 8) + m's hi (lo) 16 bytes
-        uint32_t* const base =
-            a.parts + ((int64_t)T * nball + kb) * 512 + 4 * (16 * (k >> 3) + m) + (k & 7) / 2;
-        base[0] = hv | (ho << 16);
-        base[256] = lv | (lo << 16);
-    }
-    if (k == 0) a.inv[split_inv_index(T, m, nball, kb)] = sinv;
-}
-
-
 __device__ __forceinline__ f4 mfma_f32(float x, float y, const f4& acc) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, acc, 0, 0, 0);
-}
-
-// Dimensions 4c .. 4c + 3 of head h of row r's attention output from lane c
-// of a 16-lane row (every lane of the wave takes part; nothing stored past
-// n_rows): to out, or split as attn_store does (block 2h + c / 8, its largest
-// magnitude over 8 lanes).
-__device__ __forceinline__ void attn_store4(const AttnArgs& a, int n_rows, int r, int h, int c,
-                                            const f4& o) {
-    if (!a.parts) {
-        if (r < n_rows)
-            *reinterpret_cast<f4*>(a.out + (int64_t)r * a.n_head * kHeadDim + h * kHeadDim + 4 * c) = o;
-        return;
-    }
-    float mx = fmaxf(fmaxf(fabsf(o[0]), fabsf(o[1])), fmaxf(fabsf(o[2]), fabsf(o[3])));
-#pragma unroll
-    for (int x = 1; x < 8; x <<= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-    if (r >= n_rows) return;
-    float sc, sinv;
-    split_scale(mx, sc, sinv);
-    uint32_t hi[2], lo[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float y0 = __fmul_rn(o[2 * i], sc), y1 = __fmul_rn(o[2 * i + 1], sc);
-        const _Float16 h0 = (_Float16)y0, h1 = (_Float16)y1;
-        hi[i] = __builtin_bit_cast(uint32_t, split_h2{h0, h1});
-        lo[i] = __builtin_bit_cast(uint32_t, split_h2{(_Float16)__fsub_rn(y0, (float)h0),
-                                                      (_Float16)__fsub_rn(y1, (float)h1)});
-    }
-    const int nball = a.n_head * kHeadDim / 32, kb = 2 * h + (c >> 3), T = r >> 4, m = r & 15;
-    // values 4 (c % 8) .. of the block: half (c & 1) of group (c % 8) / 2
-    uint32_t* const d =
-        a.parts + ((int64_t)T * nball + kb) * 512 + 4 * (16 * ((c & 7) >> 1) + m) + 2 * (c & 1);
-    *reinterpret_cast<uint2*>(d) = make_uint2(hi[0], hi[1]);
-    *reinterpret_cast<uint2*>(d + 256) = make_uint2(lo[0], lo[1]);
-    if ((c & 7) == 0) a.inv[split_inv_index(T, m, nball, kb)] = sinv;
 }
 
 // Prefill: every row's k and v stored at its slot and position before any
@@ -409,7 +340,7 @@ __global__ __launch_bounds__(kAttnWaves * kHeadDim) void t3_attn(AttnArgs a) {
     const int lane = tid & 63, w = tid >> 6;
     const int n = a.n_head * kHeadDim;
     if (!a.act[r]) {
-        if (tid < kHeadDim) attn_store(a, r, h, tid, 0.0f);
+        if (tid < kHeadDim) attn_store(a.o, r, h, tid, 0.0f);
         return;
     }
     const int pos = a.positions[r];
@@ -522,7 +453,7 @@ __global__ __launch_bounds__(kAttnWaves * kHeadDim) void t3_attn(AttnArgs a) {
             st = __fadd_rn(st, __fmul_rn(red[kAttnWaves + q], f));
             at = __fadd_rn(at, __fmul_rn(part[q][lane], f));
         }
-        attn_store(a, r, h, lane, __fdiv_rn(at, st));
+        attn_store(a.o, r, h, lane, __fdiv_rn(at, st));
     }
 }
 
@@ -721,7 +652,7 @@ __global__ __launch_bounds__(4 * kHeadDim) void t3_attn_tile(AttnArgs a, int n_r
             f4 x;
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) x[dt] = on ? __fdiv_rn(o[dt][v], sv) : 0.0f;
-            attn_store4(a, n_rows, __shfl(row, 4 * g + v), h, c, x);
+            attn_store4(a.o, n_rows, __shfl(row, 4 * g + v), h, c, x);
         }
     } else {
         // wave w joins the four waves' rows 4 g + w
@@ -751,7 +682,7 @@ __global__ __launch_bounds__(4 * kHeadDim) void t3_attn_tile(AttnArgs a, int n_r
         const bool on = __shfl((int)real, i) != 0;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) at[dt] = on ? __fdiv_rn(at[dt], st) : 0.0f;
-        attn_store4(a, n_rows, __shfl(row, i), h, c, at);
+        attn_store4(a.o, n_rows, __shfl(row, i), h, c, at);
     }
 }
 
@@ -924,9 +855,8 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
     aa.positions = positions;
     aa.act = act;
     aa.slots = slots;
-    aa.out = att;
-    aa.parts = mc ? sparts : nullptr;  // c_attn has read them by then
-    aa.inv = sinv;
+    // split: c_attn has read the parts by then
+    aa.o = AttnOut{att, n, mc ? sparts : nullptr, sinv, m.n_head};
     aa.scale = 0.125f;  // 1 / sqrt(64)
     const size_t lds = t3_attn_lds(c.n_ctx);
     // the prompt pass's rows in groups of one slot each (one row or one slot
