@@ -324,6 +324,9 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.cbx_t3_prefill.restype = ctypes.c_int
     lib.cbx_t3_prefill.argtypes = [vp, ctypes.POINTER(T3Model), i32, vp, i32, vp, vp, vp,
                                    ctypes.POINTER(T3Cache), vp, vp]
+    lib.cbx_t3_kv.restype = ctypes.c_int
+    lib.cbx_t3_kv.argtypes = [vp, ctypes.POINTER(T3Model), ctypes.POINTER(KvCache),
+                              ctypes.POINTER(KvStreams), ctypes.POINTER(KvRows), vp, vp, vp, vp]
     lib.cbx_kv_tile_rows.restype = i32
     lib.cbx_kv_tile_rows.argtypes = [i32, i32]
     lib.cbx_kv_build.restype = ctypes.c_int
@@ -667,6 +670,23 @@ class Sampler:
         _check(self.lib.cbx_t3_prefill(self.handle, ctypes.byref(model), slots.numel(),
                                        _ptr(slots), k_cache.shape[0], _ptr(tokens), _ptr(inputs),
                                        _ptr(positions), ctypes.byref(c), _ptr(hidden), st))
+
+    def t3_kv(self, model, cache, streams, rows, hidden, *, tokens=None, inputs=None,
+              stream=None):
+        """cbx_t3_kv: the transformer on rows planned by kv_build, over a paged
+        cache: tokens int32 [n_rows] or inputs float32 [n_rows, n_embd], hidden
+        [n_rows, n_embd] out."""
+        import torch
+        n, f = rows.n_rows, torch.float32
+        dev = self._one_call("t3_kv", streams, rows)
+        if cache._tensors[0].device != dev:
+            raise ValueError("t3_kv: the cache is on another device")
+        self._check_kv("t3_kv", dev, hidden=(hidden, f, (n, model.n_embd)),
+                       tokens=(tokens, torch.int32, (n,)), inputs=(inputs, f, (n, model.n_embd)))
+        st = _stream_ptr() if stream is None else ctypes.c_void_p(stream)
+        _check(self.lib.cbx_t3_kv(self.handle, ctypes.byref(model), ctypes.byref(cache),
+                                  ctypes.byref(streams), ctypes.byref(rows), _ptr(tokens),
+                                  _ptr(inputs), _ptr(hidden), st))
 
     # -- paged caches (include/cbx_kv.h) ----------------------------------------
     @staticmethod

@@ -562,81 +562,6 @@ int cbx_head_decode_step(cbx_sampler* s, const cbx_head* h, const cbx_batch* b,
 }  // extern "C"
 
 namespace {
-// cbx_t3_step and cbx_t3_prefill (slots set): the checks and the launch.
-int t3_run(const char* fn, cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows,
-           const int32_t* tokens, const float* inputs, int32_t* positions, const int32_t* state,
-           const int32_t* slots, int32_t n_slots, const cbx_t3_cache* cache, float* hidden,
-           void* stream) {
-    if (!s || !m || !cache) return fail(CBX_ERR_INVALID, "%s: NULL handle, model or cache", fn);
-    if (n_rows < 1) return fail(CBX_ERR_INVALID, "%s: n_rows %d", fn, n_rows);
-    if (m->n_layer < 1 || m->n_layer > 256 || !m->layers)
-        return fail(CBX_ERR_INVALID, "%s: n_layer %d or NULL layers", fn, m->n_layer);
-    if (m->n_embd < 1 || m->n_embd > 4096 || !cbx::t3_shape_ok(m->n_embd, m->n_head))
-        return fail(CBX_ERR_UNSUPPORTED,
-                    "%s: n_embd %d, n_head %d (heads of 64, n_embd in {256..1024 by 256, 1536, "
-                    "2048, 3072, 4096})", fn, m->n_embd, m->n_head);
-    if (cbx::wtype_block_bytes(m->wtype) == 0)
-        return fail(CBX_ERR_INVALID, "%s: unknown wtype %d", fn, m->wtype);
-    if (!(m->eps >= 0.0f) || !m->wpe || !m->ln_f_g || !m->ln_f_b || m->n_pos < 1 ||
-        (!inputs && (!tokens || !m->speech_emb || m->n_speech_vocab < 1)))
-        return fail(CBX_ERR_INVALID, "%s: eps, wpe, ln_f, n_pos or the embedding missing", fn);
-    for (int l = 0; l < m->n_layer; ++l) {
-        const cbx_t3_layer& L = m->layers[l];
-        if (!L.ln_1_g || !L.ln_1_b || !L.attn_w || !L.attn_b || !L.attn_proj_w ||
-            !L.attn_proj_b || !L.ln_2_g || !L.ln_2_b || !L.fc_w || !L.fc_b || !L.fc_proj_w ||
-            !L.fc_proj_b)
-            return fail(CBX_ERR_INVALID, "%s: layer %d has a NULL tensor", fn, l);
-    }
-    if (!cache->k || !cache->v || cache->n_ctx < 1 || cache->n_ctx > m->n_pos)
-        return fail(CBX_ERR_INVALID, "%s: cache k/v NULL or n_ctx %d outside [1, n_pos]", fn,
-                    cache->n_ctx);
-    if (cbx::t3_attn_lds(cache->n_ctx) + 2048 > s->lds_limit)
-        return fail(CBX_ERR_UNSUPPORTED, "%s: n_ctx %d: the attention's LDS exceeds the device's",
-                    fn, cache->n_ctx);
-    if (!positions || !hidden) return fail(CBX_ERR_INVALID, "%s: NULL positions or hidden", fn);
-    // the matrix kernels' buffer descriptors address rows in 32 bits
-    if ((int64_t)n_rows * 4 * m->n_embd * 4 > 0x7fffffffLL)
-        return fail(CBX_ERR_UNSUPPORTED, "%s: %d rows past 2 GiB of activations", fn, n_rows);
-    DeviceGuard g(s->device);
-    const size_t need = cbx::t3_workspace_bytes(n_rows, m->n_embd);
-    if (need > s->t3_bytes) {
-        CBX_HIP(hipDeviceSynchronize());
-        CBX_HIP(hipFree(s->d_t3));
-        s->d_t3 = nullptr;
-        s->t3_bytes = 0;
-        CBX_HIP(hipMalloc(&s->d_t3, need));
-        s->t3_bytes = need;
-    }
-    CBX_HIP(cbx::launch_t3_step(*m, n_rows, tokens, inputs, positions, state, slots, n_slots,
-                                *cache, hidden, s->d_t3, (hipStream_t)stream));
-    return CBX_OK;
-}
-}  // namespace
-
-extern "C" {
-
-int cbx_t3_step(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows, const int32_t* tokens,
-                const float* inputs, int32_t* positions, const int32_t* state,
-                const cbx_t3_cache* cache, float* hidden, void* stream) {
-    return t3_run("cbx_t3_step", s, m, n_rows, tokens, inputs, positions, state, nullptr, 0,
-                  cache, hidden, stream);
-}
-
-int cbx_t3_prefill(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows, const int32_t* slots,
-                   int32_t n_slots, const int32_t* tokens, const float* inputs,
-                   const int32_t* positions, const cbx_t3_cache* cache, float* hidden,
-                   void* stream) {
-    if (!slots || n_slots < 1)
-        return fail(CBX_ERR_INVALID, "cbx_t3_prefill: NULL slots or n_slots %d", n_slots);
-    // positions are read, not advanced, in the prefill form
-    return t3_run("cbx_t3_prefill", s, m, n_rows, tokens, inputs, const_cast<int32_t*>(positions),
-                  nullptr, slots, n_slots, cache, hidden, stream);
-}
-
-
-}  // extern "C"
-
-namespace {
 bool kv_page_ok(int32_t page_size) {
     return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
 }
@@ -758,5 +683,117 @@ int cbx_kv_attend(cbx_sampler* s, const cbx_kv_attn* a, void* stream) {
     CBX_HIP(cbx::launch_kv_attend(*a, nullptr, nullptr, (hipStream_t)stream));
     return CBX_OK;
 }
+
+}  // extern "C"
+
+namespace {
+// cbx_t3_step, cbx_t3_prefill (slots set) and cbx_t3_kv (kv set: the paged
+// cache, streams and rows): the checks and the launch.
+int t3_run(const char* fn, cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows,
+           const int32_t* tokens, const float* inputs, int32_t* positions, const int32_t* state,
+           const int32_t* slots, int32_t n_slots, const cbx_t3_cache* cache, float* hidden,
+           void* stream, const cbx_kv_attn* kv = nullptr) {
+    if (!s || !m || !cache) return fail(CBX_ERR_INVALID, "%s: NULL handle, model or cache", fn);
+    if (n_rows < 1) return fail(CBX_ERR_INVALID, "%s: n_rows %d", fn, n_rows);
+    if (m->n_layer < 1 || m->n_layer > 256 || !m->layers)
+        return fail(CBX_ERR_INVALID, "%s: n_layer %d or NULL layers", fn, m->n_layer);
+    if (m->n_embd < 1 || m->n_embd > 4096 || !cbx::t3_shape_ok(m->n_embd, m->n_head))
+        return fail(CBX_ERR_UNSUPPORTED,
+                    "%s: n_embd %d, n_head %d (heads of 64, n_embd in {256..1024 by 256, 1536, "
+                    "2048, 3072, 4096})", fn, m->n_embd, m->n_head);
+    if (cbx::wtype_block_bytes(m->wtype) == 0)
+        return fail(CBX_ERR_INVALID, "%s: unknown wtype %d", fn, m->wtype);
+    if (!(m->eps >= 0.0f) || !m->wpe || !m->ln_f_g || !m->ln_f_b || m->n_pos < 1 ||
+        (!inputs && (!tokens || !m->speech_emb || m->n_speech_vocab < 1)))
+        return fail(CBX_ERR_INVALID, "%s: eps, wpe, ln_f, n_pos or the embedding missing", fn);
+    for (int l = 0; l < m->n_layer; ++l) {
+        const cbx_t3_layer& L = m->layers[l];
+        if (!L.ln_1_g || !L.ln_1_b || !L.attn_w || !L.attn_b || !L.attn_proj_w ||
+            !L.attn_proj_b || !L.ln_2_g || !L.ln_2_b || !L.fc_w || !L.fc_b || !L.fc_proj_w ||
+            !L.fc_proj_b)
+            return fail(CBX_ERR_INVALID, "%s: layer %d has a NULL tensor", fn, l);
+    }
+    if (!kv && (!cache->k || !cache->v || cache->n_ctx < 1 || cache->n_ctx > m->n_pos))
+        return fail(CBX_ERR_INVALID, "%s: cache k/v NULL or n_ctx %d outside [1, n_pos]", fn,
+                    cache->n_ctx);
+    if (cbx::t3_attn_lds(cache->n_ctx) + 2048 > s->lds_limit)
+        return fail(CBX_ERR_UNSUPPORTED, "%s: n_ctx %d: the attention's LDS exceeds the device's",
+                    fn, cache->n_ctx);
+    if (!positions || !hidden) return fail(CBX_ERR_INVALID, "%s: NULL positions or hidden", fn);
+    // the matrix kernels' buffer descriptors address rows in 32 bits
+    if ((int64_t)n_rows * 4 * m->n_embd * 4 > 0x7fffffffLL)
+        return fail(CBX_ERR_UNSUPPORTED, "%s: %d rows past 2 GiB of activations", fn, n_rows);
+    cbx_kv_attn a;
+    size_t kv_bytes = 0;
+    if (kv) {
+        a = *kv;
+        a.n_head = m->n_head;
+        a.ld_q = a.ld_kv = 3 * m->n_embd;
+        a.ld_out = m->n_embd;
+        a.scale = 0.125f;             // 1 / sqrt(64)
+        // the workspace's rows stand here, layer by layer; not NULL for the checks
+        a.q = a.k = a.v = a.out = static_cast<float*>(a.cache->k);
+        const int rc = check_kv_attn(fn, &a);
+        if (rc != CBX_OK) return rc;
+        if (a.cache->n_layer != m->n_layer || a.cache->n_head != m->n_head)
+            return fail(CBX_ERR_INVALID, "%s: a cache of %d layers and %d heads, the model has %d, %d",
+                        fn, a.cache->n_layer, a.cache->n_head, m->n_layer, m->n_head);
+        kv_bytes = cbx::kv_workspace_bytes(a);
+    }
+    DeviceGuard g(s->device);
+    const size_t body = cbx::t3_workspace_bytes(n_rows, m->n_embd), need = body + kv_bytes;
+    if (need > s->t3_bytes) {
+        CBX_HIP(hipDeviceSynchronize());
+        CBX_HIP(hipFree(s->d_t3));
+        s->d_t3 = nullptr;
+        s->t3_bytes = 0;
+        CBX_HIP(hipMalloc(&s->d_t3, need));
+        s->t3_bytes = need;
+    }
+    if (kv) a.workspace = static_cast<char*>(s->d_t3) + body;
+    CBX_HIP(cbx::launch_t3_step(*m, n_rows, tokens, inputs, positions, state, slots, n_slots,
+                                *cache, hidden, s->d_t3, (hipStream_t)stream, kv ? &a : nullptr));
+    return CBX_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int cbx_t3_step(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows, const int32_t* tokens,
+                const float* inputs, int32_t* positions, const int32_t* state,
+                const cbx_t3_cache* cache, float* hidden, void* stream) {
+    return t3_run("cbx_t3_step", s, m, n_rows, tokens, inputs, positions, state, nullptr, 0,
+                  cache, hidden, stream);
+}
+
+int cbx_t3_prefill(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows, const int32_t* slots,
+                   int32_t n_slots, const int32_t* tokens, const float* inputs,
+                   const int32_t* positions, const cbx_t3_cache* cache, float* hidden,
+                   void* stream) {
+    if (!slots || n_slots < 1)
+        return fail(CBX_ERR_INVALID, "cbx_t3_prefill: NULL slots or n_slots %d", n_slots);
+    // positions are read, not advanced, in the prefill form
+    return t3_run("cbx_t3_prefill", s, m, n_rows, tokens, inputs, const_cast<int32_t*>(positions),
+                  nullptr, slots, n_slots, cache, hidden, stream);
+}
+
+int cbx_t3_kv(cbx_sampler* s, const cbx_t3_model* m, const cbx_kv_cache* cache,
+              const cbx_kv_streams* streams, const cbx_kv_rows* rows, const int32_t* tokens,
+              const float* inputs, float* hidden, void* stream) {
+    const char* fn = "cbx_t3_kv";
+    if (!s || !m || !cache) return fail(CBX_ERR_INVALID, "%s: NULL handle, model or cache", fn);
+    const int rc = check_kv(fn, streams, rows, cache->page_size);
+    if (rc != CBX_OK) return rc;
+    if (!hidden) return fail(CBX_ERR_INVALID, "%s: NULL hidden", fn);
+    cbx_kv_attn a = {};
+    a.cache = cache;
+    a.streams = streams;
+    a.rows = rows;
+    const cbx_t3_cache none = {nullptr, nullptr, m->n_pos};
+    // rows take part by their slots; positions are the plan's, only read
+    return t3_run(fn, s, m, rows->n_rows, tokens, inputs, rows->position, nullptr, rows->slot,
+                  cache->n_pages * cache->page_size, &none, hidden, stream, &a);
+}
+
 
 }  // extern "C"

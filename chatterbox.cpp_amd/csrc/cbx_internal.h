@@ -217,10 +217,12 @@ bool t3_shape_ok(int32_t n_embd, int32_t n_head);
 size_t t3_attn_lds(int32_t n_ctx);
 size_t t3_workspace_bytes(int32_t n_rows, int32_t n_embd);
 // slots set: the prefill form (cbx_t3_prefill); positions are not advanced.
+// kv set: the paged cache's rows instead of c's (slots their places in it; its
+// workspace given, q, k, v and out filled in here).
 hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* tokens,
                           const float* inputs, int32_t* positions, const int32_t* state,
                           const int32_t* slots, int32_t n_slots, const cbx_t3_cache& c,
-                          float* hidden, void* ws, hipStream_t st);
+                          float* hidden, void* ws, hipStream_t st, const cbx_kv_attn* kv);
 
 // The paged cache (cbx_kv_plan.hip, cbx_kv_attn.hip), arguments already checked.
 // kMaxKvStreams: a plan's one workgroup holds 16 streams a thread and, for a

@@ -795,10 +795,11 @@ size_t t3_workspace_bytes(int32_t n_rows, int32_t n_embd) {
 hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* tokens,
                           const float* inputs, int32_t* positions, const int32_t* state,
                           const int32_t* slots, int32_t n_slots, const cbx_t3_cache& c,
-                          float* hidden, void* ws, hipStream_t st) {
+                          float* hidden, void* ws, hipStream_t st, const cbx_kv_attn* kv) {
     // slots set: a prefill (rows of one stream may share a call: their k and v
-    // are stored before the attention, and positions do not advance)
-    const bool prefill = slots != nullptr;
+    // are stored before the attention, and positions do not advance), or the
+    // paged cache's rows (cbx_kv_attn.hip stores and attends)
+    const bool prefill = slots != nullptr && !kv;
     const int n = m.n_embd;
     const size_t row = (size_t)n_rows * n;
     float* x = static_cast<float*>(ws);
@@ -808,7 +809,7 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
     float* qkv = y + kMaxKSplit * row;
     float* f = qkv + 3 * row;
     int32_t* act = reinterpret_cast<int32_t*>(f + 4 * row);
-    const bool wide = !prefill && t3_attn_wide(n_rows, m.n_head);
+    const bool wide = !slots && t3_attn_wide(n_rows, m.n_head);
     void* split = reinterpret_cast<char*>(act) + ((size_t)n_rows * 4 + 255) / 256 * 256;
     void* split2 = static_cast<char*>(split) + t3_split_bytes(n_rows, n);
     int32_t* const groups =
@@ -887,20 +888,20 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
     // the products of rows already split, from `in`
     auto product = [&](const void* w, const float* b, float* out, int n_out, int n_in,
                        const void* in, int kz, bool gelu, void* out_split,
-                       const KvOut& kv = KvOut{}) {
+                       const KvOut& kv_out = KvOut{}) {
         return head_uses_tiles(n_rows, n_in) && kz == 1
                    ? launch_head_tiles(w, m.wtype, b, out, n_out, n_rows, n_out, n_in, in, unpacked,
-                                       st, gelu, out_split, kv)
+                                       st, gelu, out_split, kv_out)
                    : launch_head_presplit(w, m.wtype, b, out, n_out, n_rows, n_out, n_in, in, st,
-                                          kz, gelu, out_split, kv);
+                                          kz, gelu, out_split, kv_out);
     };
     for (int l = 0; l < m.n_layer; ++l) {
         const cbx_t3_layer& L = m.layers[l];
         if (mc) {
-            const KvOut kv = prefill ? KvOut{c.k, c.v, positions, slots, act, l, m.n_layer,
+            const KvOut place = prefill ? KvOut{c.k, c.v, positions, slots, act, l, m.n_layer,
                                              m.n_head, c.n_ctx}
-                                     : KvOut{};
-            e = product(L.attn_w, L.attn_b, qkv, 3 * n, n, split, 1, false, nullptr, kv);
+                                        : KvOut{};
+            e = product(L.attn_w, L.attn_b, qkv, 3 * n, n, split, 1, false, nullptr, place);
         } else if (fold && l > 0) {  // the previous layer's residual + this ln_1
             gn.x_in = xcur;
             gn.x_out = xcur = xcur == x ? xalt : x;
@@ -914,7 +915,15 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
         }
         if (e != hipSuccess) return e;
         aa.layer = l;
-        if (prefill) {
+        if (kv) {
+            cbx_kv_attn ka = *kv;
+            ka.layer = l;
+            ka.q = qkv;
+            ka.k = qkv + n;
+            ka.v = qkv + 2 * n;
+            ka.out = att;
+            if ((e = launch_kv_attend(ka, aa.o.parts, aa.o.inv, st)) != hipSuccess) return e;
+        } else if (prefill) {
             if (!mc) {
                 hipLaunchKernelGGL(t3_kv_append, dim3((unsigned)n_rows, (unsigned)m.n_head),
                                    dim3(kHeadDim), 0, st, aa);
@@ -979,7 +988,7 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
         nc.out = last ? hidden : u;
         nc.parts = mc && !last ? sparts : nullptr;
         nc.positions = positions;
-        nc.advance = last && !prefill ? 1 : 0;
+        nc.advance = last && !slots ? 1 : 0;
         if ((e = launch_norm(nc, n_rows, st)) != hipSuccess) return e;
     }
     return hipSuccess;

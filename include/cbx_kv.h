@@ -12,8 +12,7 @@
  *
  * A serving loop: cbx_kv_build plans a call's rows (pages taken, where each
  * row's key and value go), then for every layer cbx_kv_attend stores them and
- * attends; cbx_t3_step_kv and cbx_t3_prefill_kv (cbx_t3.h) run the whole
- * transformer on such rows.
+ * attends; cbx_t3_kv (cbx_t3.h) runs the whole transformer on such rows.
  *
  * Device pointers throughout, but for the structures themselves; every call
  * is asynchronous on `stream`, allocates nothing and holds nothing in the

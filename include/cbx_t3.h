@@ -22,6 +22,7 @@
 
 #include <stdint.h>
 
+#include "cbx_kv.h"
 #include "cbx_sampler.h"
 
 #ifdef __cplusplus
@@ -111,6 +112,24 @@ int cbx_t3_prefill(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows,
                    const int32_t* slots, int32_t n_slots, const int32_t* tokens,
                    const float* inputs, const int32_t* positions,
                    const cbx_t3_cache* cache, float* hidden, void* stream);
+
+/* Rows planned by cbx_kv_build through the transformer, on a paged cache of
+ * the model's layers and heads (cbx_kv.h): in the step form the decode step of
+ * every stream that has a row (cbx_t3_step's), in the prompt form any number of
+ * positions of each stream in one call (cbx_t3_prefill's), behind the prefix it
+ * shares.  Row r's input is speech id tokens[r] at position[r] (or, with
+ * `inputs`, the embedded row inputs[r][0, n_embd)); its k and v go to slot[r]
+ * in every layer, and ln_f's output to hidden[r].  The plan has advanced the
+ * streams already: positions are only read.  Rows without a slot give zero
+ * rows; so does a row whose position is outside [0, n_pos) or whose token is
+ * outside [0, n_speech_vocab): the keys stored for it are a zero input's.
+ * tile_rows is cbx_kv_tile_rows(n_head, n_head).  Sums and products as in
+ * cbx_t3_step; the handle holds the workspace, so calls on one handle are
+ * ordered on one stream.  Replaces eval_step and eval_prompt
+ * (main.cpp:643-710) up to ln_f. */
+int cbx_t3_kv(cbx_sampler* s, const cbx_t3_model* m, const cbx_kv_cache* cache,
+              const cbx_kv_streams* streams, const cbx_kv_rows* rows, const int32_t* tokens,
+              const float* inputs, float* hidden, void* stream);
 
 #ifdef __cplusplus
 }
