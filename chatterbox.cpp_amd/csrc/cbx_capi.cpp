@@ -619,7 +619,7 @@ int check_kv_attn(const char* fn, const cbx_kv_attn* a) {
         return fail(CBX_ERR_INVALID, "%s: NULL q or out, or one of k and v", fn);
     const int64_t width = (int64_t)64 * a->n_head;
     if (a->ld_q < width || a->ld_out < width || a->ld_q % 4 || a->ld_out % 4 ||
-        (a->k && (a->ld_kv < (int64_t)64 * c.n_head || a->ld_kv % 4)))
+        (a->k && (a->ld_kv < (int64_t)64 * c.n_head || a->ld_kv % 4 || a->ld_kv > 0x7fffffffLL)))
         return fail(CBX_ERR_INVALID, "%s: row strides %lld, %lld, %lld", fn, (long long)a->ld_q,
                     (long long)a->ld_out, (long long)a->ld_kv);
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||

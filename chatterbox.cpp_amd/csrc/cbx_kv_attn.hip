@@ -58,6 +58,7 @@ struct KvArgs {
     const float* v;
     int64_t ld_kv;
     int32_t n_head, group;  // query heads, of them per key head
+    uint32_t over_group;    // x / group = x * over_group >> 16 for x < 128
     float scale;
     AttnOut o;
     // parts of rows cut over workgroups, [part][n_rows][n_head]: (m, s) and
@@ -68,14 +69,18 @@ struct KvArgs {
     int32_t n_own, n_shared;
 };
 
+__device__ __forceinline__ int over_group(const KvArgs& a, int x) {
+    return (int)((uint32_t)x * a.over_group >> 16);
+}
+
 // Stream i's prefix as cbx_kv_build counts it: its table's stream and the
 // positions shared (0: none).
 __device__ __forceinline__ int prefix_of(const KvArgs& a, int i, int& plen) {
     plen = 0;
     if (!a.parent || i < a.n_prefix || i >= a.n_streams) return -1;
-    const int p = a.parent[i];
+    const int p = a.parent[i], n = a.prefix_len[i];  // both loads before the first use
     if (p < 0 || p >= a.n_prefix) return -1;
-    plen = min(max(a.prefix_len[i], 0), a.max_pages << a.shift);
+    plen = min(max(n, 0), a.max_pages << a.shift);
     return p;
 }
 
@@ -98,6 +103,13 @@ __device__ __forceinline__ f4 load4(const T* base, uint32_t row, int d) {
         const h4 x = *reinterpret_cast<const h4*>(p);
         return f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
     }
+}
+
+template <class T>
+__device__ __forceinline__ void store4(T* base, uint32_t row, int d, const f4& x) {
+    T* const p = base + ((uint64_t)row << 6) + d;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<f4*>(p) = x;
+    else *reinterpret_cast<h4*>(p) = h4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
 }
 
 // ------------------------------------------------------------------ step form
@@ -349,82 +361,347 @@ __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
 
 // ------------------------------------------------------------------ tiles
 
-// The prompt form's new rows to their slots, before any row attends.
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+// Values as parts that the 16-bit matrix cores multiply exactly (products in
+// fp32), two to a dword.
+//  * fp32 caches: three bf16 parts, each the leading 8 bits of what the ones
+//    before leave: x = h + m + l to the last bit wherever l is not subnormal,
+//    at any magnitude.  Of the nine products of two such values six are formed;
+//    m l, l m and l l are below 2^-23 of the whole.
+//  * fp16 caches: keys and values as they are; queries and weights two fp16
+//    parts, x = hi + lo to 2^-22.
+// The fp32 matrix instructions run on the vector units' own multipliers, 32
+// cycles for a 16x16x4, and nothing else runs beside them: with them the
+// softmax's vector work came on top (us, prefix part of 512 rows x 2001 keys x
+// 16 heads: 67; prompts of 64 x 129-383 rows: 236).
 template <class T>
-__global__ __launch_bounds__(256) void kv_store(KvArgs a) {
-    const int r = blockIdx.x, s = a.slot[r];
-    if (s < 0 || (s >> a.shift) >= a.n_pages) return;
-    for (int i = threadIdx.x; i < a.n_kv * 16; i += 256) {
-        const int kvh = i >> 4, d = 4 * (i & 15);
-        const uint64_t at = ((uint64_t)cache_row(a, s >> a.shift, kvh, s) << 6) + d;
-        const f4 k = *reinterpret_cast<const f4*>(a.k + r * a.ld_kv + kvh * kDim + d);
-        const f4 v = *reinterpret_cast<const f4*>(a.v + r * a.ld_kv + kvh * kDim + d);
-        T* const kc = static_cast<T*>(const_cast<void*>(a.kc)) + at;
-        T* const vc = static_cast<T*>(const_cast<void*>(a.vc)) + at;
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<f4*>(kc) = k;
-            *reinterpret_cast<f4*>(vc) = v;
-        } else {
-            *reinterpret_cast<h4*>(kc) = h4{(T)k[0], (T)k[1], (T)k[2], (T)k[3]};
-            *reinterpret_cast<h4*>(vc) = h4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+struct Parts;
+template <>
+struct Parts<float> {
+    static constexpr int kKv = 3, kQ = 3, kProducts = 6;
+    __device__ static constexpr int kv(int i) { constexpr int x[6] = {2, 1, 0, 1, 0, 0}; return x[i]; }
+    __device__ static constexpr int q(int i) { constexpr int x[6] = {0, 1, 2, 0, 1, 0}; return x[i]; }
+    // parts of two neighbours
+    __device__ static __forceinline__ void split(float x, float y, uint32_t (&p)[3]) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, x), v = __builtin_bit_cast(uint32_t, y);
+            p[i] = __builtin_amdgcn_perm(v, u, 0x07060302u);  // their upper halves
+            x = __fsub_rn(x, __builtin_bit_cast(float, u & 0xffff0000u));
+            y = __fsub_rn(y, __builtin_bit_cast(float, v & 0xffff0000u));
         }
     }
+    __device__ static __forceinline__ f4 mfma(const u4& x, const u4& y, const f4& acc) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x),
+                                                       __builtin_bit_cast(b8, y), acc, 0, 0, 0);
+    }
+};
+template <>
+struct Parts<_Float16> {
+    static constexpr int kKv = 1, kQ = 2, kProducts = 2;
+    __device__ static constexpr int kv(int) { return 0; }
+    __device__ static constexpr int q(int i) { return 1 - i; }
+    __device__ static __forceinline__ void split(float x, float y, uint32_t (&p)[2]) {
+        const _Float16 a = (_Float16)x, b = (_Float16)y;
+        p[0] = __builtin_bit_cast(uint32_t, split_h2{a, b});
+        p[1] = __builtin_bit_cast(uint32_t, split_h2{(_Float16)__fsub_rn(x, (float)a),
+                                                     (_Float16)__fsub_rn(y, (float)b)});
+    }
+    __device__ static __forceinline__ f4 mfma(const u4& x, const u4& y, const f4& acc) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x),
+                                                      __builtin_bit_cast(h8, y), acc, 0, 0, 0);
+    }
+};
+
+// Four keys of one dimension from rows of 16-bit values in LDS: of each 16
+// lanes, lane 4 r + q names 4 dimensions (quarter q of 16) of key r, and lane i
+// gets dimension i of keys 0 .. 3.
+__device__ __forceinline__ u2 read_transposed(const char* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    return __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p)));
 }
 
-__device__ __forceinline__ f4 mfma_f32(float x, float y, const f4& acc) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, acc, 0, 0, 0);
+// A tile's walk: [0, plen) in pre_t's pages, the rest in own_t's, from
+// position fresh0 on the call's own rows from row fresh_row (which its streams
+// store in this launch).
+struct Walk {
+    const int32_t* pre_t;
+    const int32_t* own_t;
+    int plen, end, fresh0, fresh_row;
+};
+
+// The table entry that says where key j < end is (the new rows': their slot);
+// read without a branch, so that nothing waits for it before it is used.
+__device__ __forceinline__ int entry_of(const KvArgs& a, const Walk& k, int j) {
+    const int x = min(j, k.end - 1);
+    const bool theirs = x < k.plen;
+    const int place = theirs ? x : x - k.plen;
+    const int32_t* p = (theirs ? k.pre_t : k.own_t) + (place >> a.shift);
+    if (x >= k.fresh0) p = a.slot + min(k.fresh_row + (x - k.fresh0), a.n_rows - 1);
+    return *p;
 }
 
-// A wave takes 16 (row, head) pairs of a tile and one key head and walks its
-// keys 32 at a time with v_mfma_f32_16x16x4_f32.
-//  * Scores transposed, S^T = K Q^T: lane (g = l / 16, c = l % 16) feeds key c
-//    and pair c at dimensions 16 cc + 4 g + e (step (cc, e)), and holds pair
-//    c's scores at keys 4 g + v: its own pair's limit, maximum and sum, joined
-//    over g by two exchanges.
-//  * P V: those exponentials are the A operand as they stand (pair c, step v:
-//    key 4 g + v), V[4 g + v][4 c ..] the B operand, one 16-byte load for four
-//    output tiles, so lane (g, c) ends with pairs 4 g + v at dimensions
-//    4 c .. 4 c + 3.
+// 16 (row, head) pairs of a tile a wave, on the matrix cores.  The keys and
+// values of a stage (kKeys of them) are loaded once for the workgroup, through
+// registers into LDS (as parts) while the stage before is computed on; their
+// places are looked up a stage before that.
+//  * Scores transposed, S^T = K Q^T, 32 keys at a time: lane (g = l / 16,
+//    c = l % 16) ends with pair c's scores at keys 4 g + i and 16 + 4 g + i, so
+//    a pair's limit, maximum, sum and rescaling are its own lanes', joined over
+//    g by two exchanges.
+//  * Outputs transposed, O^T = V^T P^T: those weights are the second operand as
+//    they stand, V's operand is read transposed (tile dt: dimension 16 dt +
+//    4 g + i).
+// With fp16 parts q is scaled by a power of two per pair (its largest magnitude
+// to [2^14, 2^15)) and the weights by 2^14 (their largest is 1), so that parts
+// lose nothing to subnormals that the sum would notice.
 // A key that a pair does not see has weight 0, and 0 times a V that is not
-// finite would reach the pair: where some pair does not see all 32 keys, such
-// values are looked for, and if there are any, added pair by pair with the
-// unseen keys' V at 0.
-// KS = 4: the workgroup's four waves take the same pairs and every fourth
-// 32 keys, joined through LDS; KS = 1: each wave its own pairs.
+// finite would reach the pair: a stage that holds such values is noted as it is
+// stored, and where some pair does not see all of 32 keys of it, they are added
+// pair by pair with the unseen keys' V at 0.
+// SPLIT: the four waves take the same 16 pairs and 32 keys of a stage each,
+// joined through LDS (few rows); else each wave its own pairs and all keys.
 // PART: the step form's prefixes: keys cut over blockIdx.y, parts stored.
-template <class T, int KS, bool PART>
-__global__ __launch_bounds__(256) void kv_tiles(KvArgs a) {
-    constexpr int KT = 2;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+template <class T, bool SPLIT, bool PART>
+__global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
+    constexpr bool F16 = sizeof(T) == 2;
+    constexpr int kKeys = SPLIT ? 128 : 32;
+    using P = Parts<T>;
+    constexpr int kCh = kDim * sizeof(T) / 16;       // 16-byte chunks of a row in memory
+    constexpr int kStep = 256 / kCh;                 // rows that the workgroup loads at a time
+    constexpr int kU = kKeys / kStep;                // rows a thread loads of a stage
+    constexpr int kPer = 16 / sizeof(T);             // values of a chunk
+    constexpr int kPad = kDim + 4;                   // a pair's outputs in LDS
+    constexpr int kPart = kKeys * kDim * 2, kStage = P::kKv * kPart;  // bytes: a part, K or V
+    constexpr int kBufs = SPLIT ? 1 : 2;
+    // [buffer][K, V][part], then the outputs in their place
+    constexpr int kOut = 4 * 16 * kPad * 4, kLds = 2 * kBufs * kStage;
+    __shared__ __align__(16) char lds[kLds > kOut ? kLds : kOut];
+    // of a stage (three in turn: one read, one written, one cleared): whether
+    // values are not finite, and the keys without a place, a bit each
+    __shared__ int odd[3];
+    __shared__ uint32_t gone[3][kKeys / 32];
+    __shared__ float join_m[4][16], join_s[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int g = lane >> 4, c = lane & 15;
     const int kvh = blockIdx.x % a.n_kv, unit = blockIdx.x / a.n_kv;
     const T* const kc = static_cast<const T*>(a.kc);
     const T* const vc = static_cast<const T*>(a.vc);
-    if (!PART) {  // rows behind the last
+    int4 tile = a.tiles[SPLIT ? unit / 4 : unit];
+    tile = make_int4(__builtin_amdgcn_readfirstlane(tile.x), __builtin_amdgcn_readfirstlane(tile.y),
+                     __builtin_amdgcn_readfirstlane(tile.z), __builtin_amdgcn_readfirstlane(tile.w));
+    const int p0 = SPLIT ? 16 * (unit % 4) : 0;      // the workgroup's first pair
+    const int count = min(tile.z, a.tile_rows);
+    const int pairs = tile.x >= 0 && tile.x < a.n_streams ? count * a.group : 0;
+    const auto dead_rows = [&]() {  // rows behind the last give zeros
+        if (PART) return;
         const int total = a.row_start[a.n_streams];
         for (int64_t r = (int64_t)max(total, 0) + blockIdx.x; r < a.n_rows; r += gridDim.x)
             for (int h = w; h < a.n_head; h += 4) attn_store(a.o, (int)r, h, lane, 0.0f);
+    };
+    if (p0 >= pairs) {
+        dead_rows();
+        return;
     }
-    const int4 tile = a.tiles[KS == 1 ? unit : unit / 4];
-    const int p = 16 * (KS == 1 ? w : unit % 4) + c;
-    const int count = min(tile.z, a.tile_rows);
+    const int p = p0 + (SPLIT ? 0 : 16 * w) + c;
     const int first = min(max(tile.y, 0), a.n_rows);
-    const int at = first + p / a.group, h = kvh * a.group + p % a.group;
-    bool real = tile.x >= 0 && tile.x < a.n_streams && p < count * a.group && at < a.n_rows;
+    const int local = over_group(a, p), at = first + local, h = kvh * a.group + p - local * a.group;
+    bool real = p < pairs && at < a.n_rows;
     int row = -1;
     if (real) row = PART ? a.order[at] : at;
     real = real && row >= 0 && row < a.n_rows;
-    if (!__ballot(real)) return;  // a whole workgroup, or no barrier follows
     const int rc = real ? row : 0;
-    // lim: the last key the pair sees
-    int plen = 0, pre = -1, lim;
+    // the walk, and lim, the last key the pair sees
+    const int cap = a.max_pages << a.shift;
+    Walk k;
+    int lim, begin = 0;
+    k.own_t = a.tables + (int64_t)tile.x * a.max_pages;
+    k.pre_t = k.own_t;
+    k.fresh0 = INT32_MAX;
+    k.fresh_row = 0;
     if (PART) {
+        k.plen = 0;
         prefix_of(a, rc, lim);
         lim = real ? lim - 1 : -1;
+        // this workgroup's keys, the same for all pairs of the tile
+        const int keys = min(max(tile.w, 0), cap);
+        const int used = min(a.n_shared, (keys + kMinPart - 1) / kMinPart);
+        const int size = used > 0 ? ((keys + used - 1) / used + 31) / 32 * 32 : 0;
+        begin = min((int)blockIdx.y * size, keys);
+        k.end = min(begin + size, keys);
     } else {
-        pre = prefix_of(a, tile.x, plen);
-        lim = real ? min(a.position[rc], plen + (a.max_pages << a.shift) - 1) : -1;
+        const int pre = prefix_of(a, tile.x, k.plen);
+        if (pre >= 0) k.pre_t = a.tables + (int64_t)pre * a.max_pages;
+        lim = real ? min(a.position[rc], k.plen + cap - 1) : -1;
+        k.end = min(tile.w, k.plen + cap);
+        if (a.k) {  // the stream's first new row and its position
+            k.fresh_row = min(max(a.row_start[tile.x], 0), first);
+            k.fresh0 = max(a.position[min(first, a.n_rows - 1)] - (first - k.fresh_row), 0);
+        }
+        // with SPLIT, the pairs' last key ends the walk
+        if (SPLIT) {
+            const int end_row = first + over_group(a, min(p0 + 15, pairs - 1));
+            k.end = min(k.end, a.position[min(end_row, a.n_rows - 1)] + 1);
+        }
     }
+    k.end = __builtin_amdgcn_readfirstlane(k.end);  // as the whole workgroup has it
+    k.plen = __builtin_amdgcn_readfirstlane(k.plen);
+    k.fresh0 = __builtin_amdgcn_readfirstlane(k.fresh0);
+    k.fresh_row = __builtin_amdgcn_readfirstlane(k.fresh_row);
+    // a part in LDS: rows of eight 16-byte chunks, a row's in an order of its own
+    // so that 16 rows' reads of one chunk fall in different banks
+    const auto chunk_at = [&](char* base, int r, int ch) {
+        return base + (r * 8 + (ch ^ (r >> 1 & 7))) * 16;
+    };
+    const int ch = tid % kCh, r0 = tid / kCh;
+    int next[kU];
+    // a stage's loads, nothing of them used before they are stored: a chunk of
+    // K and V each, the fp16 forms' new rows (fp32) in two
+    constexpr int kLoads = F16 && !PART ? 2 : 1;
+    u4 kr[kU][kLoads], vr[kU][kLoads];
+    uint32_t none = 0, fresh = 0;  // rows that have no place, and new ones: a bit each
+    // the tile's own new rows (with SPLIT, those that begin among its pairs) go to
+    // their slots as they are staged: rows [own0, own1) of the call
+    uint32_t to[kU];
+    const int own0 = PART || !a.k ? 0 : first + over_group(a, p0 + a.group - 1);
+    const int own1 = PART || !a.k ? 0 : min(first + min(SPLIT ? over_group(a, p0 + 15 + a.group) : count, count), a.n_rows);
+    const auto look = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) next[u] = entry_of(a, k, j0 + r0 + u * kStep);
+    };
+    // the stage from j0 on, its entries in next
+    const auto load = [&](int j0) {
+        none = fresh = 0;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int j = j0 + r0 + u * kStep, place = j < k.plen ? j : j - k.plen;
+            const bool own = !PART && j >= k.fresh0;
+            const uint32_t row = cache_row(a, own ? next[u] >> a.shift : next[u], kvh, place);
+            if (j >= k.end || row == kNoRow) none |= 1u << u;
+            uint64_t from = ((uint64_t)(row == kNoRow ? 0 : row) << 6) + kPer * ch;
+            const void *ks = kc, *vs = vc;
+            to[u] = kNoRow;
+            if (own) {
+                fresh |= 1u << u;
+                const int r = min(k.fresh_row + (j - k.fresh0), a.n_rows - 1);
+                if (j < k.end && r >= own0 && r < own1) to[u] = row;
+                from = (uint64_t)r * (uint32_t)a.ld_kv + kvh * kDim + kPer * ch;
+                ks = a.k;
+                vs = a.v;
+                if (F16) from *= 2;  // in fp16 units
+            }
+            kr[u][0] = *reinterpret_cast<const u4*>(static_cast<const T*>(ks) + from);
+            vr[u][0] = *reinterpret_cast<const u4*>(static_cast<const T*>(vs) + from);
+            if constexpr (F16 && !PART) {
+                if (own) {
+                    kr[u][1] = *reinterpret_cast<const u4*>(static_cast<const T*>(ks) + from + 8);
+                    vr[u][1] = *reinterpret_cast<const u4*>(static_cast<const T*>(vs) + from + 8);
+                }
+            }
+        }
+    };
+    const auto store = [&](int b, int slot) {
+        char* const kb = lds + 2 * b * kStage;
+        if (__ballot(none != 0)) {
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+                if (none >> u & 1) {
+                    if (ch == 0) atomicOr(&gone[slot][(r0 + u * kStep) >> 5], 1u << ((r0 + u * kStep) & 31));
+                    kr[u][0] = vr[u][0] = u4{0, 0, 0, 0};
+                    if (F16 && !PART) kr[u][kLoads - 1] = vr[u][kLoads - 1] = u4{0, 0, 0, 0};
+                }
+        }
+        // 0 times every value: NaN once one is not finite
+        float odd4 = 0.0f;
+        split_h2 odd8 = split_h2{(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+            const int r = r0 + u * kStep;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // K, V
+                u4 y = x ? vr[u][0] : kr[u][0];
+                if constexpr (F16 && !PART) {
+                    if (fresh >> u & 1) {  // rounded as the cache will hold them
+                        const f4 lo = __builtin_bit_cast(f4, y);
+                        const f4 hi = __builtin_bit_cast(f4, x ? vr[u][1] : kr[u][1]);
+                        y = __builtin_bit_cast(u4, h8{(_Float16)lo[0], (_Float16)lo[1], (_Float16)lo[2],
+                                                      (_Float16)lo[3], (_Float16)hi[0], (_Float16)hi[1],
+                                                      (_Float16)hi[2], (_Float16)hi[3]});
+                    }
+                }
+                if (!PART && to[u] != kNoRow)
+                    *reinterpret_cast<u4*>(const_cast<T*>(x ? vc : kc) + ((uint64_t)to[u] << 6) + kPer * ch) = y;
+                if constexpr (F16) {
+                    if (x) {
+                        const split_h2 zero = split_h2{(_Float16)0.0f, (_Float16)0.0f};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            odd8 = __builtin_elementwise_fma(__builtin_bit_cast(split_h2, (uint32_t)y[i]), zero, odd8);
+                    }
+                    *reinterpret_cast<u4*>(chunk_at(kb + x * kStage, r, ch)) = y;
+                } else {
+                    const f4 z = __builtin_bit_cast(f4, y);
+                    if (x) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) odd4 = __fmaf_rn(z[i], 0.0f, odd4);
+                    }
+                    uint32_t lo[P::kQ], hi[P::kQ];
+                    P::split(z[0], z[1], lo);
+                    P::split(z[2], z[3], hi);
+#pragma unroll
+                    for (int i = 0; i < P::kKv; ++i)
+                        *reinterpret_cast<u2*>(chunk_at(kb + x * kStage + i * kPart, r, ch >> 1) +
+                                               8 * (ch & 1)) = u2{lo[i], hi[i]};
+                }
+            }
+        }
+        if (F16) odd4 = (float)odd8[0] + (float)odd8[1];
+        if (odd4 != odd4) odd[slot] = 1;
+    };
+    // q, scaled: dimensions 32 ks + 8 g .. of pair c, in parts; a score is the
+    // matrix cores' times unit_of; c2: to powers of two
+    u4 qp[2][P::kQ];
+    float unit_of = 1.0f, c2 = kLog2e;
+    {
+        const float* const qr = a.q + rc * a.ld_q + (real ? h : 0) * kDim;
+        float x[2][8], mx = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const f4 v = *reinterpret_cast<const f4*>(qr + 32 * ks + 8 * g + e) * a.scale;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[ks][e + i] = v[i];
+                    mx = fmaxf(mx, fabsf(v[i]));
+                }
+            }
+        float sc = 1.0f;
+        if (F16) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            split_scale(mx, sc, unit_of);
+            c2 = __fmul_rn(kLog2e, unit_of);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t y[P::kQ];
+                P::split(__fmul_rn(x[ks][2 * e], sc), __fmul_rn(x[ks][2 * e + 1], sc), y);
+#pragma unroll
+                for (int i = 0; i < P::kQ; ++i) qp[ks][i][e] = y[i];
+            }
+    }
+    constexpr float kUp = F16 ? 14.0f : 0.0f;  // the weights' scale, a power of two
+    f4 o[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, s = 0.0f;  // m as the matrix cores give the scores
     int last = lim, least = real ? lim : INT32_MAX;
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) {
@@ -433,180 +710,205 @@ __global__ __launch_bounds__(256) void kv_tiles(KvArgs a) {
     }
     last = __builtin_amdgcn_readfirstlane(last);
     least = __builtin_amdgcn_readfirstlane(least);
-    int begin = 0, end = last + 1;
-    if (PART) {  // this workgroup's keys, the same for all pairs of the tile
-        const int keys = min(max(tile.w, 0), a.max_pages << a.shift);
-        const int used = min(a.n_shared, (keys + kMinPart - 1) / kMinPart);
-        const int size = used > 0 ? ((keys + used - 1) / used + 15) / 16 * 16 : 0;
-        begin = min((int)blockIdx.y * size, keys);
-        end = min(end, min(begin + size, keys));
-    }
-    f4 q[4], o[4];
-    {
-        const float* const qr = a.q + rc * a.ld_q + (real ? h : 0) * kDim + 4 * g;
+
+    // 32 keys from j0 on: rows b .. of a buffer
+    const auto compute = [&](int buf, int slot, int b, int j0) {
+        char* const kb = lds + 2 * buf * kStage;
+        char* const vb = kb + kStage;
+        const uint32_t miss = __builtin_amdgcn_readfirstlane(gone[slot][b >> 5]);
+        f4 x[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-            q[cc] = *reinterpret_cast<const f4*>(qr + 16 * cc) * a.scale;
-            o[cc] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int ks = 0; ks < 2; ++ks) {
+            u4 y[2][P::kKv];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < P::kKv; ++i)
+                    y[kt][i] = *reinterpret_cast<const u4*>(
+                        chunk_at(kb + i * kPart, b + 16 * kt + c, 4 * ks + g));
+#pragma unroll
+            for (int i = 0; i < P::kProducts; ++i)
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+                    x[kt] = P::mfma(y[kt][P::kv(i)], qp[ks][P::q(i)], x[kt]);
         }
-    }
-    const int32_t* const own_t = a.tables + (int64_t)min(max(tile.x, 0), a.n_streams - 1) * a.max_pages;
-    const int32_t* const pre_t = a.tables + (int64_t)max(pre, 0) * a.max_pages;
-    float m = -INFINITY, s = 0.0f;
-    for (int j0 = begin + (KS == 1 ? 0 : 16 * KT * w); j0 < end; j0 += 16 * KT * KS) {
-        // lane l: where key j0 + l % 32 is (keys past the end: the last's)
-        const int jl = min(j0 + (lane & 31), end - 1);
-        const bool theirs = jl < plen;
-        const int place = theirs ? jl : jl - plen;
-        const uint32_t where =
-            cache_row(a, (theirs ? pre_t : own_t)[place >> a.shift], kvh, place);
-        // the keys with a page, a bit each
-        const uint32_t paged = (uint32_t)__ballot(where != kNoRow);
-        f4 kk[KT][4], vv[KT][4], x[KT];
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-            uint32_t kr = (uint32_t)__shfl((int)where, 16 * kt + c);
-            kr = kr == kNoRow ? 0 : kr;
-#pragma unroll
-            for (int cc = 0; cc < 4; ++cc) kk[kt][cc] = load4(kc, kr, 16 * cc + 4 * g);
-        }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                uint32_t vr = (uint32_t)__shfl((int)where, 16 * kt + 4 * g + v);
-                const bool none = vr == kNoRow;
-                vv[kt][v] = load4(vc, none ? 0 : vr, 4 * c);
-                if (none) vv[kt][v] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) x[kt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt) x[kt] = mfma_f32(kk[kt][cc][e], q[cc][e], x[kt]);
-        const auto seen = [&](int kt, int v) {
-            const int k = 16 * kt + 4 * g + v;
-            return j0 + k <= lim && j0 + k < end && (paged >> k & 1);
+        // whether some pair of the wave does not see all 32
+        const bool partial = j0 + 31 > least || j0 + 32 > k.end || miss != 0;
+        // the keys up to `limit` that are there, a bit each
+        const auto seen = [&](int limit) {
+            const int n = min(limit, k.end - 1) - j0;
+            return (n < 0 ? 0u : n >= 31 ? ~0u : (2u << n) - 1) & ~miss;
         };
+        if (partial) {
+            const uint32_t see = seen(lim) >> (4 * g);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(see >> (16 * kt + i) & 1)) x[kt][i] = -INFINITY;
+        }
         float bm = -INFINITY;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-                if (seen(kt, v)) bm = fmaxf(bm, x[kt][v]);
+        for (int i = 0; i < 4; ++i) bm = fmaxf(bm, fmaxf(x[0][i], x[1][i]));
         bm = fmaxf(bm, __shfl_xor(bm, 16));
         bm = fmaxf(bm, __shfl_xor(bm, 32));
         if (__ballot(bm > m)) {
             const float nm = fmaxf(m, bm);
-            const float f = m == -INFINITY ? 0.0f : exp_of(__fsub_rn(m, nm));
+            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, nm), c2));
             s = __fmul_rn(s, f);
             m = nm;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float fv = __shfl(f, 4 * g + v);  // pair 4 g + v's
+            for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-                for (int dt = 0; dt < 4; ++dt) o[dt][v] = __fmul_rn(o[dt][v], fv);
-            }
+                for (int i = 0; i < 4; ++i) o[dt][i] = __fmul_rn(o[dt][i], f);
         }
+        // weights; unseen keys and scores of -inf have none
+        const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const bool on = seen(kt, v) && !(x[kt][v] == -INFINITY);
-                x[kt][v] = on ? exp_of(__fsub_rn(x[kt][v], m)) : 0.0f;
-                s = __fadd_rn(s, x[kt][v]);
+            for (int i = 0; i < 4; ++i) {
+                x[kt][i] = __builtin_amdgcn_exp2f(__fmaf_rn(__fsub_rn(x[kt][i], base), c2, kUp));
+                s = __fadd_rn(s, x[kt][i]);
             }
-        bool plain = true;
-        if (j0 + 16 * KT - 1 > least || j0 + 16 * KT > end) {
-            float z = 0.0f;  // NaN once a value is not finite
+        const bool plain = !(partial && __builtin_amdgcn_readfirstlane(odd[slot]));
+        u4 wp[P::kQ];  // the weights' parts, the lane's eight keys
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+        for (int e = 0; e < 4; ++e) {
+            uint32_t y[P::kQ];
+            P::split(x[e >> 1][2 * (e & 1)], x[e >> 1][2 * (e & 1) + 1], y);
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-#pragma unroll
-                    for (int dt = 0; dt < 4; ++dt) z = __fmaf_rn(vv[kt][v][dt], 0.0f, z);
-            plain = __ballot(z != z) == 0;
+            for (int i = 0; i < P::kQ; ++i) wp[i][e] = y[i];
         }
+        const auto value = [&](int dt, int i) {  // part i of dimension 16 dt + c of the lane's keys
+            u4 y;
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const u2 z = read_transposed(chunk_at(vb + i * kPart, b + 16 * kt + 4 * g + (c >> 2),
+                                                      2 * dt + (c >> 1 & 1)) + 8 * (c & 1));
+                y[2 * kt] = z[0];
+                y[2 * kt + 1] = z[1];
+            }
+            return y;
+        };
         if (plain) {
 #pragma unroll
-            for (int kt = 0; kt < KT; ++kt)
+            for (int dt = 0; dt < 4; ++dt) {
+                u4 y[P::kKv];
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
+                for (int i = 0; i < P::kKv; ++i) y[i] = value(dt, i);
 #pragma unroll
-                    for (int dt = 0; dt < 4; ++dt) o[dt] = mfma_f32(x[kt][v], vv[kt][v][dt], o[dt]);
+                for (int i = 0; i < P::kProducts; ++i) o[dt] = P::mfma(y[P::kv(i)], wp[P::q(i)], o[dt]);
+            }
         } else {
 #pragma unroll 1
-            for (int i = 0; i < 16; ++i) {
-                const int li = __builtin_amdgcn_readlane(lim, i);
+            for (int n = 0; n < 16; ++n) {
+                const uint32_t see = seen(__builtin_amdgcn_readlane(lim, n)) >> (4 * g);
 #pragma unroll
                 for (int dt = 0; dt < 4; ++dt) {
+                    u4 y[P::kKv];
+#pragma unroll
+                    for (int i = 0; i < P::kKv; ++i) {
+                        y[i] = value(dt, i);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t two = see >> (16 * (e >> 1) + 2 * (e & 1));
+                            y[i][e] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+                        }
+                    }
                     f4 add = o[dt];
 #pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            const int j = j0 + 16 * kt + 4 * g + v;
-                            add = mfma_f32(x[kt][v], j <= li && j < end ? vv[kt][v][dt] : 0.0f, add);
-                        }
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        if (4 * g + v == i) o[dt][v] = add[v];
+                    for (int i = 0; i < P::kProducts; ++i) add = P::mfma(y[P::kv(i)], wp[P::q(i)], add);
+                    if (c == n) o[dt] = add;
                 }
             }
         }
+    };
+
+    const int stages = (max(k.end - begin, 0) + kKeys - 1) / kKeys;
+    if (tid < 3) {
+        odd[tid] = 0;
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) gone[tid][i] = 0;
+    }
+    __syncthreads();
+    if (stages > 0) {
+        look(begin);
+        load(begin);
+        look(begin + kKeys);
+        store(0, 0);
+    }
+    __syncthreads();
+    for (int t = 0; t < stages; ++t) {
+        const int j0 = begin + t * kKeys, slot = t % 3;
+        const bool more = t + 1 < stages;
+        if (more) {
+            load(j0 + kKeys);
+            look(j0 + 2 * kKeys);
+        }
+        if (tid == 0) {
+            odd[(t + 2) % 3] = 0;
+#pragma unroll
+            for (int i = 0; i < kKeys / 32; ++i) gone[(t + 2) % 3][i] = 0;
+        }
+#pragma unroll 1
+        for (int b = SPLIT ? 32 * w : 0; b < kKeys; b += SPLIT ? kKeys : 32)
+            if (j0 + b <= last && j0 + b < k.end) compute(kBufs == 2 ? t & 1 : 0, slot, b, j0 + b);
+        if (kBufs == 1) __syncthreads();
+        if (more) store(kBufs == 2 ? (t + 1) & 1 : 0, (t + 1) % 3);
+        __syncthreads();
     }
     s = __fadd_rn(s, __shfl_xor(s, 16));  // the pair's sum over its four lanes
     s = __fadd_rn(s, __shfl_xor(s, 32));
-    // pair i's (m, s, o): a part, or the row's outputs
-    const auto store = [&](int i, float pm, float psum, const f4& po) {
+    // through LDS into rows: [16 w + pair][dimension]
+    float* const os = reinterpret_cast<float*>(lds) + 16 * w * kPad;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        *reinterpret_cast<f4*>(os + c * kPad + 16 * i + 4 * g) = o[i];
+    }
+    if (g == 0) {
+        join_m[w][c] = __fmul_rn(m, unit_of);
+        join_s[w][c] = s;
+    }
+    __syncthreads();
+    // lane (g, c): dimensions 4 c .. of pair i
+    const auto finish = [&](int i, float pm, float ps, const f4& po) {
         const int ri = __shfl(real ? row : a.n_rows, i), hi = __shfl(h, i);
         if (PART) {
             if (ri >= a.n_rows) return;
+            constexpr float kDown = F16 ? 1.0f / 16384.0f : 1.0f;
             const int64_t to = ((int64_t)(a.n_own + blockIdx.y) * a.n_rows + ri) * a.n_head + hi;
-            if (c == 0) a.part_ms[to] = float2{pm, psum};
-            *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * c) = po;
+            if (c == 0) a.part_ms[to] = float2{pm, __fmul_rn(ps, kDown)};
+            *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * c) = po * kDown;
         } else {
-            f4 y;
-#pragma unroll
-            for (int dt = 0; dt < 4; ++dt) y[dt] = psum == 0.0f ? 0.0f : __fdiv_rn(po[dt], psum);
-            attn_store4(a.o, a.n_rows, ri, hi, c, y);
+            const float over = ps == 0.0f ? 0.0f : __fdiv_rn(1.0f, ps);
+            attn_store4(a.o, a.n_rows, ri, hi, c, po * over);
         }
     };
-    if constexpr (KS == 1) {
+    if constexpr (!SPLIT) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-            store(4 * g + v, __shfl(m, 4 * g + v), __shfl(s, 4 * g + v),
-                  f4{o[0][v], o[1][v], o[2][v], o[3][v]});
-    } else {
-        // wave w joins the four waves' pairs 4 g + w
-        __shared__ f4 os[KS][4][64];
-        __shared__ float ms[KS][16], ss[KS][16];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) os[w][v][lane] = f4{o[0][v], o[1][v], o[2][v], o[3][v]};
-        if (g == 0) {
-            ms[w][c] = m;
-            ss[w][c] = s;
+        for (int t = 0; t < 4; ++t) {
+            const int i = 4 * t + g;
+            finish(i, join_m[w][i], join_s[w][i], *reinterpret_cast<const f4*>(os + i * kPad + 4 * c));
         }
-        __syncthreads();
-        const int i = 4 * g + w;
-        float M = ms[0][i];
+    } else {  // wave w joins the four waves' pairs 4 w + g
+        const int i = 4 * w + g;
+        float M = join_m[0][i];
 #pragma unroll
-        for (int x = 1; x < KS; ++x) M = fmaxf(M, ms[x][i]);
+        for (int x = 1; x < 4; ++x) M = fmaxf(M, join_m[x][i]);
         float st = 0.0f;
         f4 ot = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-            const float f = ms[x][i] == -INFINITY ? 0.0f : exp_of(__fsub_rn(ms[x][i], M));
-            st = __fadd_rn(st, __fmul_rn(ss[x][i], f));
-            const f4 ov = os[x][w][lane];
+        for (int x = 0; x < 4; ++x) {
+            const float mx = join_m[x][i], f = mx == -INFINITY ? 0.0f : exp_of(__fsub_rn(mx, M));
+            st = __fadd_rn(st, __fmul_rn(join_s[x][i], f));
+            const f4 ov = *reinterpret_cast<const f4*>(reinterpret_cast<float*>(lds) + (16 * x + i) * kPad + 4 * c);
 #pragma unroll
-            for (int dt = 0; dt < 4; ++dt) ot[dt] = __fadd_rn(ot[dt], __fmul_rn(ov[dt], f));
+            for (int e = 0; e < 4; ++e) ot[e] = __fadd_rn(ot[e], __fmul_rn(ov[e], f));
         }
-        store(i, M, st, ot);
+        finish(i, M, st, ot);
     }
+    dead_rows();
 }
 
 // ------------------------------------------------------------------ launches
@@ -634,7 +936,7 @@ Cut cut_of(const cbx_kv_attn& a) {
     if (tiles) {
         const int64_t t = (int64_t)a.rows->n_tiles * a.cache->n_head;
         const int64_t most = std::min<int64_t>(32, (cap + kMinPart - 1) / kMinPart);
-        c.shared = (int)std::min(std::max<int64_t>((1024 + t - 1) / t, 1), most);
+        c.shared = (int)std::min(std::max<int64_t>((768 + t / 2) / t, 1), most);
         c.own = (int)own;
     } else {
         c.own = own > 1 ? (int)own : 0;
@@ -663,20 +965,14 @@ hipError_t launch_tiles(const KvArgs& a, bool part, hipStream_t st) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
         return hipGetLastError();
     };
-    if (part) return split ? go(kv_tiles<T, 4, true>) : go(kv_tiles<T, 1, true>);
-    return split ? go(kv_tiles<T, 4, false>) : go(kv_tiles<T, 1, false>);
+    if (part) return split ? go(kv_tiles<T, true, true>) : go(kv_tiles<T, false, true>);
+    return split ? go(kv_tiles<T, true, false>) : go(kv_tiles<T, false, false>);
 }
 
 template <class T>
 hipError_t launch(const KvArgs& a, bool step, hipStream_t st) {
     hipError_t e;
-    if (!step) {
-        if (a.k) {
-            hipLaunchKernelGGL(kv_store<T>, dim3((unsigned)a.n_rows), dim3(256), 0, st, a);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-        }
-        return launch_tiles<T>(a, false, st);
-    }
+    if (!step) return launch_tiles<T>(a, false, st);
     if (a.n_shared && (e = launch_tiles<T>(a, true, st)) != hipSuccess) return e;
     if ((e = launch_rows<T>(a, st)) != hipSuccess || !a.n_own) return e;
     const int64_t waves = (int64_t)a.n_rows * a.n_head;
@@ -726,6 +1022,7 @@ hipError_t launch_kv_attend(const cbx_kv_attn& c, uint32_t* parts, float* inv, h
     a.ld_kv = c.ld_kv;
     a.n_head = c.n_head;
     a.group = c.n_head / p.n_head;
+    a.over_group = 65536 / a.group + 1;
     a.scale = c.scale;
     a.o = AttnOut{c.out, c.ld_out, parts, inv, c.n_head};
     const uint64_t n = (uint64_t)(cut.own + cut.shared) * r.n_rows * c.n_head;
