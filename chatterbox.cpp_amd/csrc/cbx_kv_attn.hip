@@ -67,6 +67,7 @@ struct KvArgs {
     float2* part_ms;
     float* part_o;
     int32_t n_own, n_shared;
+    int32_t min_part;  // keys that a part of a row's own has at least, where there are more
 };
 
 __device__ __forceinline__ int over_group(const KvArgs& a, int x) {
@@ -114,69 +115,51 @@ __device__ __forceinline__ void store4(T* base, uint32_t row, int d, const f4& x
 
 // ------------------------------------------------------------------ step form
 
-constexpr int kRowWaves = 4;
-// Pages whose ids a workgroup holds at once.
-constexpr int kIds = 512;
-// Keys that a part of a row's own has at least (below, the row takes fewer).
+// Keys that a part has at least, where there are more.
 constexpr int kMinPart = 64;
 
-// One part of one row's keys, for G of its key head's query heads.  The part's
-// page ids go to LDS; the waves take batches of keys in turn, LPK lanes to a
-// key (16 bytes of it each), kU keys per lane in flight; each lane group keeps
-// a running (m, s, o) of its keys, joined over the groups and waves in a fixed
-// order.  The row's new k and v come from its input row, stored on the way.
-template <class T, int G>
-__global__ __launch_bounds__(64 * kRowWaves) void kv_rows(KvArgs a) {
-    constexpr int DPL = 16 / sizeof(T), LPK = kDim / DPL, KPI = 64 / LPK;  // dims a lane, lanes a key
-    constexpr int kU = G > 2 ? 4 : 6;
-    __shared__ int32_t ids[kIds];
-    __shared__ __align__(16) float new_k[kDim], new_v[kDim];
-    __shared__ float red_m[kRowWaves][G], red_s[kRowWaves][G];
-    __shared__ __align__(16) float red_o[kRowWaves][G][kDim];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int chunks = (a.group + G - 1) / G;
-    const int r = blockIdx.x / (a.n_kv * chunks), y = blockIdx.x % (a.n_kv * chunks);
+// Sixteen bytes of a cache row as they are, and their values.
+template <class T>
+struct Chunk;
+template <>
+struct Chunk<float> {
+    static constexpr int kN = 4;
+    typedef f4 Raw;
+    __device__ static __forceinline__ float at(const Raw& x, int i) { return x[i]; }
+};
+template <>
+struct Chunk<_Float16> {
+    static constexpr int kN = 8;
+    typedef h8 Raw;
+    __device__ static __forceinline__ float at(const Raw& x, int i) { return (float)x[i]; }
+};
+
+// One part of one row's keys, for G of its key head's query heads, by W waves
+// (4: a workgroup; 1: the workgroup's waves take a head each, with no barrier).
+// LPK lanes to a key, 16 bytes of it each, kU keys per lane in flight; the page
+// ids of 64 pages are held by the wave's lanes, and handed over by an exchange.
+// Each lane group keeps a running (m, s, o) of its keys, joined over the groups
+// and waves in a fixed order.  The row's new k and v come from its input row,
+// stored on the way.
+template <class T, int G, int W>
+__global__ __launch_bounds__(256) void kv_rows(KvArgs a) {
+    using C = Chunk<T>;
+    constexpr int DPL = C::kN, LPK = kDim / DPL, KPI = 64 / LPK;  // dims a lane, lanes a key
+    constexpr int kU = G > 2 || sizeof(T) == 2 ? 4 : 6;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int chunks = (a.group + G - 1) / G, per_row = a.n_kv * chunks;
+    const int64_t unit = W == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + w;
+    if (unit >= (int64_t)a.n_rows * per_row) return;
+    const int r = (int)(unit / per_row), y = (int)(unit % per_row);
     const int kvh = y / chunks, g0 = y % chunks * G, h0 = kvh * a.group + g0;
     const int ng = min(G, a.group - g0), part = blockIdx.y;
+    const int sub = lane / LPK, d0 = lane % LPK * DPL;
     const int pos = a.position[r];
+    const int slot = a.k ? a.slot[r] : -1;
     int plen;
     const int pre = prefix_of(a, r, plen);
-    // keys [c0, c1) of the row: its own alone where tiles take the prefix
-    const int cap = a.max_pages << a.shift;
-    const int lo = a.tiles ? min(plen, pos + 1) : 0;
-    const int end = min(pos + 1, plen + cap);
-    const int L = max(end - lo, 0), used = min(a.n_own > 0 ? a.n_own : 1, (L + kMinPart - 1) / kMinPart);
-    const int size = used > 0 ? (L + used - 1) / used : 0;
-    const int c0 = lo + part * size, c1 = part < used ? min(c0 + size, end) : c0;
-    if (c0 >= c1) {  // no keys
-        if (a.n_own > 0) {
-            if (tid < ng)
-                a.part_ms[((int64_t)part * a.n_rows + r) * a.n_head + h0 + tid] = float2{-INFINITY, 0.0f};
-        } else if (w == 0) {
-            for (int g = 0; g < ng; ++g) attn_store(a.o, r, h0 + g, lane, 0.0f);
-        }
-        return;
-    }
-    const T* const kc = static_cast<const T*>(a.kc);
-    const T* const vc = static_cast<const T*>(a.vc);
-    const bool has_new = a.k != nullptr && pos >= c0 && pos < c1;
-    if (has_new && w == 0) {
-        // rounded as the cache holds it
-        const T kn = (T)a.k[r * a.ld_kv + kvh * kDim + lane];
-        const T vn = (T)a.v[r * a.ld_kv + kvh * kDim + lane];
-        new_k[lane] = (float)kn;
-        new_v[lane] = (float)vn;
-        const int s = a.slot[r];
-        const uint32_t row = cache_row(a, s < 0 ? -1 : s >> a.shift, kvh, s);
-        if (g0 == 0 && row != kNoRow) {
-            const_cast<T*>(kc)[((uint64_t)row << 6) + lane] = kn;
-            const_cast<T*>(vc)[((uint64_t)row << 6) + lane] = vn;
-        }
-    }
-    // whether the new position is one that the row sees
-    const bool new_ok = has_new && a.slot[r] >= 0 && (a.slot[r] >> a.shift) < a.n_pages;
-    const int sub = lane / LPK, d0 = lane % LPK * DPL;
-    float q[G][DPL], o[G][DPL], m[G], s[G];
+    // q, scaled, and the new row as the cache will hold it
+    float q[G][DPL];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         const float* const qr = a.q + r * a.ld_q + (h0 + min(g, ng - 1)) * kDim + d0;
@@ -184,80 +167,119 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv_rows(KvArgs a) {
         for (int d = 0; d < DPL; d += 4) {
             const f4 x = *reinterpret_cast<const f4*>(qr + d);
 #pragma unroll
+            for (int e = 0; e < 4; ++e) q[g][d + e] = __fmul_rn(x[e], a.scale);
+        }
+    }
+    typename C::Raw new_k{}, new_v{};
+    if (a.k) {
+        const int64_t at = r * a.ld_kv + kvh * kDim + d0;
+#pragma unroll
+        for (int d = 0; d < DPL; d += 4) {
+            const f4 x = *reinterpret_cast<const f4*>(a.k + at + d), z = *reinterpret_cast<const f4*>(a.v + at + d);
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
-                q[g][d + e] = __fmul_rn(x[e], a.scale);
-                o[g][d + e] = 0.0f;
+                new_k[d + e] = (T)x[e];
+                new_v[d + e] = (T)z[e];
             }
         }
+    }
+    // keys [c0, c1) of the row: its own alone where tiles take the prefix
+    const int cap = a.max_pages << a.shift;
+    const int lo = a.tiles ? min(plen, pos + 1) : 0;
+    const int end = min(pos + 1, plen + cap);
+    const int L = max(end - lo, 0), used = min(a.n_own > 0 ? a.n_own : 1, (L + a.min_part - 1) / a.min_part);
+    const int size = used > 0 ? (L + used - 1) / used : 0;
+    const int c0 = lo + part * size, c1 = part < used ? min(c0 + size, end) : c0;
+    const T* const kc = static_cast<const T*>(a.kc);
+    const T* const vc = static_cast<const T*>(a.vc);
+    // whether the new position is this part's, and one that the row sees
+    const bool has_new = a.k && pos >= c0 && pos < c1;
+    const uint32_t home = cache_row(a, slot < 0 ? -1 : slot >> a.shift, kvh, slot);
+    if (has_new && home != kNoRow && g0 == 0 && sub == 0 && (W == 1 || w == 0)) {
+        const uint64_t at = ((uint64_t)home << 6) + d0;
+        *reinterpret_cast<typename C::Raw*>(const_cast<T*>(kc) + at) = new_k;
+        *reinterpret_cast<typename C::Raw*>(const_cast<T*>(vc) + at) = new_v;
+    }
+    float o[G][DPL], m[G], s[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) o[g][d] = 0.0f;
         m[g] = -INFINITY;
         s[g] = 0.0f;
     }
     const int32_t* const own_t = a.tables + (int64_t)r * a.max_pages;
     const int32_t* const pre_t = a.tables + (int64_t)max(pre, 0) * a.max_pages;
-    const int ps = 1 << a.shift;
     for (int s0 = c0; s0 < c1;) {
-        // the ids of [s0, s1): the prefix's pages, then the row's own
-        const int in_pre = s0 < plen ? ((min(c1, plen) - 1) >> a.shift) - (s0 >> a.shift) + 1 : 0;
-        const int n_pre = min(in_pre, kIds);
+        // the ids of [s0, s1): the prefix's pages, then the row's own, 64 in all
         const int a0 = s0 >> a.shift, b0 = (max(s0, plen) - plen) >> a.shift;
-        int s1 = n_pre < in_pre || plen >= c1 ? min(c1, (a0 + n_pre) << a.shift)
-                                               : min((int64_t)c1, plen + (((int64_t)b0 + kIds - n_pre) << a.shift));
-        if (plen >= c1) s1 = min(s1, c1);
-        const int n_own_pages = s1 > plen ? ((s1 - 1 - plen) >> a.shift) - b0 + 1 : 0;
-        if (s0 != c0) __syncthreads();
-        for (int i = tid; i < n_pre + n_own_pages; i += 64 * kRowWaves)
-            ids[i] = i < n_pre ? pre_t[a0 + i] : own_t[b0 + i - n_pre];
-        __syncthreads();
-        for (int j0 = s0 + w * KPI * kU; j0 < s1; j0 += kRowWaves * KPI * kU) {
-            float kk[kU][DPL], vv[kU][DPL], x[kU][G];
+        const int n_pre = s0 < plen ? min(((min(c1, plen) - 1) >> a.shift) - a0 + 1, 64) : 0;
+        const int64_t reach = n_pre > 0 && (int64_t)(a0 + n_pre) << a.shift < plen
+                                  ? (int64_t)(a0 + n_pre) << a.shift
+                                  : plen + ((int64_t)(b0 + 64 - n_pre) << a.shift);
+        const int s1 = (int)min((int64_t)c1, reach);
+        const int n_ids = n_pre + (s1 > plen ? ((s1 - 1 - plen) >> a.shift) - b0 + 1 : 0);
+        const int32_t* const from = lane < n_pre ? pre_t + a0 + lane : own_t + b0 + lane - n_pre;
+        const int held = lane < n_ids ? *from : -1;
+        // a wave's batches of KPI kU keys in turn with the workgroup's
+        for (int j0 = s0 + (W == 4 ? w * KPI * kU : 0); j0 < s1; j0 += W * KPI * kU) {
+            typename C::Raw kk[kU], vv[kU];
             bool on[kU];
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 const int j = min(j0 + KPI * u + sub, s1 - 1);
                 const bool theirs = j < plen;
                 const int place = theirs ? j : j - plen;
-                const int id = ids[(place >> a.shift) - (theirs ? a0 : b0 - n_pre)];
-                const uint32_t row = cache_row(a, id, kvh, place & (ps - 1));
-                on[u] = j0 + KPI * u + sub < s1 && (has_new && j == pos ? new_ok : row != kNoRow);
-                const uint32_t at = row == kNoRow ? 0 : row;
-#pragma unroll
-                for (int d = 0; d < DPL; d += 4) {
-                    const f4 kx = load4(kc, at, d0 + d), vx = load4(vc, at, d0 + d);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        kk[u][d + e] = kx[e];
-                        vv[u][d + e] = vx[e];
-                    }
-                }
+                const int id = __shfl(held, (place >> a.shift) - (theirs ? a0 : b0 - n_pre));
+                const uint32_t row = cache_row(a, id, kvh, place);
+                on[u] = j0 + KPI * u + sub < s1 && row != kNoRow;
+                const uint64_t at = ((uint64_t)(row == kNoRow ? 0 : row) << 6) + d0;
+                kk[u] = *reinterpret_cast<const typename C::Raw*>(kc + at);
+                vv[u] = *reinterpret_cast<const typename C::Raw*>(vc + at);
             }
             if (has_new && pos >= j0 && pos < j0 + KPI * kU) {
 #pragma unroll
                 for (int u = 0; u < kU; ++u)
                     if (j0 + KPI * u + sub == pos) {
-#pragma unroll
-                        for (int d = 0; d < DPL; ++d) {
-                            kk[u][d] = new_k[d0 + d];
-                            vv[u][d] = new_v[d0 + d];
-                        }
+                        kk[u] = new_k;
+                        vv[u] = new_v;
+                        on[u] = home != kNoRow;
                     }
+            }
+            // a value that the row does not see may be anything: 0 instead
+            bool all = true;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) all = all && on[u];
+            const bool whole = __ballot(!all) == 0;
+            if (!whole) {
+#pragma unroll
+                for (int u = 0; u < kU; ++u)
+                    if (!on[u]) vv[u] = typename C::Raw{};
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                float bm = m[g];
+                float x[kU], bm = m[g];
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
                     float t = 0.0f;
 #pragma unroll
-                    for (int d = 0; d < DPL; ++d) t = __fmaf_rn(q[g][d], kk[u][d], t);
-                    t = __fadd_rn(t, dpp16<0xB1>(t));   // the key's lanes
+                    for (int d = 0; d < DPL; ++d) t = __fmaf_rn(C::at(kk[u], d), q[g][d], t);
+                    t = __fadd_rn(t, dpp16<0xB1>(t));  // the key's lanes
                     t = __fadd_rn(t, dpp16<0x4E>(t));
                     t = __fadd_rn(t, dpp16<0x141>(t));
                     if (LPK == 16) t = __fadd_rn(t, dpp16<0x140>(t));
-                    x[u][g] = t;
-                    if (on[u]) bm = fmaxf(bm, t);
+                    x[u] = t;
                 }
-                if (bm > m[g]) {
-                    const float f = exp_of(__fsub_rn(m[g], bm));  // 0 from -inf
+                if (!whole) {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u) x[u] = on[u] ? x[u] : -INFINITY;
+                }
+#pragma unroll
+                for (int u = 0; u < kU; ++u) bm = fmaxf(bm, x[u]);
+                // a key that is not there, or -inf while none is larger, has weight 0
+                const float base = bm == -INFINITY ? 0.0f : bm;
+                if (__ballot(bm > m[g])) {
+                    const float f = exp_of(__fsub_rn(m[g], base));  // 0 from -inf, 1 where it stays
                     s[g] = __fmul_rn(s[g], f);
 #pragma unroll
                     for (int d = 0; d < DPL; ++d) o[g][d] = __fmul_rn(o[g][d], f);
@@ -265,19 +287,16 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv_rows(KvArgs a) {
                 }
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    // a key that is -inf while no other is larger has no weight
-                    if (on[u] && !(x[u][g] == -INFINITY)) {
-                        const float e = exp_of(__fsub_rn(x[u][g], m[g]));
-                        s[g] = __fadd_rn(s[g], e);
+                    const float e = exp_of(__fsub_rn(x[u], base));
+                    s[g] = __fadd_rn(s[g], e);
 #pragma unroll
-                        for (int d = 0; d < DPL; ++d) o[g][d] = __fmaf_rn(e, vv[u][d], o[g][d]);
-                    }
+                    for (int d = 0; d < DPL; ++d) o[g][d] = __fmaf_rn(C::at(vv[u], d), e, o[g][d]);
                 }
             }
         }
         s0 = s1;
     }
-    // the groups of a wave, then the waves, joined in order
+    // the lane groups joined: every group ends with the wave's (m, s, o)
 #pragma unroll
     for (int g = 0; g < G; ++g) {
 #pragma unroll
@@ -292,33 +311,52 @@ __global__ __launch_bounds__(64 * kRowWaves) void kv_rows(KvArgs a) {
                 o[g][d] = __fadd_rn(__fmul_rn(o[g][d], f), __fmul_rn(__shfl_xor(o[g][d], x), fo));
             m[g] = M;
         }
-        if (lane == 0) {
-            red_m[w][g] = m[g];
-            red_s[w][g] = s[g];
-        }
-        if (sub == 0) {
-#pragma unroll
-            for (int d = 0; d < DPL; ++d) red_o[w][g][d0 + d] = o[g][d];
-        }
     }
-    __syncthreads();
-    for (int g = w; g < ng; g += kRowWaves) {
-        float M = red_m[0][g];
-#pragma unroll
-        for (int i = 1; i < kRowWaves; ++i) M = fmaxf(M, red_m[i][g]);
-        float st = 0.0f, ot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kRowWaves; ++i) {
-            const float f = red_m[i][g] == -INFINITY ? 0.0f : exp_of(__fsub_rn(red_m[i][g], M));
-            st = __fadd_rn(st, __fmul_rn(red_s[i][g], f));
-            ot = __fadd_rn(ot, __fmul_rn(red_o[i][g][lane], f));
-        }
+    // head h0 + g of the row from 64 lanes, a dimension each: a part, or the row's
+    const auto store = [&](int g, float pm, float ps, float po) {
         if (a.n_own > 0) {
             const int64_t at = ((int64_t)part * a.n_rows + r) * a.n_head + h0 + g;
-            if (lane == 0) a.part_ms[at] = float2{M, st};
-            a.part_o[at * kDim + lane] = ot;
+            if (lane == 0) a.part_ms[at] = float2{pm, ps};
+            if (c0 < c1) a.part_o[at * kDim + lane] = po;
         } else {
-            attn_store(a.o, r, h0 + g, lane, st == 0.0f ? 0.0f : __fdiv_rn(ot, st));
+            attn_store(a.o, r, h0 + g, lane, ps == 0.0f ? 0.0f : __fdiv_rn(po, ps));
+        }
+    };
+    __shared__ __align__(16) float red_o[4][G][kDim];
+    if (sub == 0) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int d = 0; d < DPL; ++d) red_o[w][g][d0 + d] = o[g][d];
+    }
+    if constexpr (W == 1) {  // wave-private: its own stores are seen in order
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+            if (g < ng) store(g, m[g], s[g], red_o[w][g][lane]);
+    } else {
+        __shared__ float red_m[4][G], red_s[4][G];
+        if (lane == 0) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                red_m[w][g] = m[g];
+                red_s[w][g] = s[g];
+            }
+        }
+        __syncthreads();
+        for (int g = w; g < ng; g += 4) {
+            float M = red_m[0][g];
+#pragma unroll
+            for (int i = 1; i < 4; ++i) M = fmaxf(M, red_m[i][g]);
+            float st = 0.0f, ot = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f = red_m[i][g] == -INFINITY ? 0.0f : exp_of(__fsub_rn(red_m[i][g], M));
+                st = __fadd_rn(st, __fmul_rn(red_s[i][g], f));
+                ot = __fadd_rn(ot, __fmul_rn(red_o[i][g][lane], f));
+            }
+            store(g, M, st, ot);
         }
     }
 }
@@ -465,15 +503,20 @@ __device__ __forceinline__ int entry_of(const KvArgs& a, const Walk& k, int j) {
 // pair by pair with the unseen keys' V at 0.
 // SPLIT: the four waves take the same 16 pairs and 32 keys of a stage each,
 // joined through LDS (few rows); else each wave its own pairs and all keys.
-// PART: the step form's prefixes: keys cut over blockIdx.y, parts stored.
-template <class T, bool SPLIT, bool PART>
+// FORM: the prompt form; the step form's prefixes, keys cut over blockIdx.y,
+// parts stored; or one row's heads of a key head against the row's keys, cut
+// likewise (where many query heads share a key head: the step form on the
+// vector units then spends its time on products).
+enum { kPrompt, kPrefix, kOneRow };
+template <class T, bool SPLIT, int FORM>
 __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
-    constexpr bool F16 = sizeof(T) == 2;
+    constexpr bool F16 = sizeof(T) == 2, PROMPT = FORM == kPrompt;
+    static_assert(SPLIT || FORM != kOneRow, "a row's heads are one wave's pairs");
     constexpr int kKeys = SPLIT ? 128 : 32;
     using P = Parts<T>;
     constexpr int kCh = kDim * sizeof(T) / 16;       // 16-byte chunks of a row in memory
     constexpr int kStep = 256 / kCh;                 // rows that the workgroup loads at a time
-    constexpr int kU = kKeys / kStep;                // rows a thread loads of a stage
+    constexpr int kU = kKeys / kStep;               // rows a thread loads of a stage
     constexpr int kPer = 16 / sizeof(T);             // values of a chunk
     constexpr int kPad = kDim + 4;                   // a pair's outputs in LDS
     constexpr int kPart = kKeys * kDim * 2, kStage = P::kKv * kPart;  // bytes: a part, K or V
@@ -491,67 +534,99 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
     const int kvh = blockIdx.x % a.n_kv, unit = blockIdx.x / a.n_kv;
     const T* const kc = static_cast<const T*>(a.kc);
     const T* const vc = static_cast<const T*>(a.vc);
-    int4 tile = a.tiles[SPLIT ? unit / 4 : unit];
-    tile = make_int4(__builtin_amdgcn_readfirstlane(tile.x), __builtin_amdgcn_readfirstlane(tile.y),
-                     __builtin_amdgcn_readfirstlane(tile.z), __builtin_amdgcn_readfirstlane(tile.w));
-    const int p0 = SPLIT ? 16 * (unit % 4) : 0;      // the workgroup's first pair
-    const int count = min(tile.z, a.tile_rows);
-    const int pairs = tile.x >= 0 && tile.x < a.n_streams ? count * a.group : 0;
     const auto dead_rows = [&]() {  // rows behind the last give zeros
-        if (PART) return;
+        if (!PROMPT) return;
         const int total = a.row_start[a.n_streams];
         for (int64_t r = (int64_t)max(total, 0) + blockIdx.x; r < a.n_rows; r += gridDim.x)
             for (int h = w; h < a.n_head; h += 4) attn_store(a.o, (int)r, h, lane, 0.0f);
     };
+    // the workgroup's rows: [first, first + count) of the call (of order, where
+    // prefixes are shared) for key stream `who`, and its first pair
+    const int subs = FORM == kOneRow ? (a.group + 15) / 16 : 4;
+    const int p0 = SPLIT ? 16 * (unit % subs) : 0;
+    int who, first, count, keys;
+    if (FORM == kOneRow) {
+        who = first = unit / subs;
+        count = 1;
+        keys = 0;
+    } else {
+        const int4 tile = a.tiles[SPLIT ? unit / 4 : unit];
+        who = __builtin_amdgcn_readfirstlane(tile.x);
+        first = min(max(__builtin_amdgcn_readfirstlane(tile.y), 0), a.n_rows);
+        count = min(__builtin_amdgcn_readfirstlane(tile.z), a.tile_rows);
+        keys = __builtin_amdgcn_readfirstlane(tile.w);
+        if (who < 0 || who >= a.n_streams) count = 0;
+    }
+    const int pairs = count * a.group;
     if (p0 >= pairs) {
         dead_rows();
         return;
     }
     const int p = p0 + (SPLIT ? 0 : 16 * w) + c;
-    const int first = min(max(tile.y, 0), a.n_rows);
     const int local = over_group(a, p), at = first + local, h = kvh * a.group + p - local * a.group;
     bool real = p < pairs && at < a.n_rows;
     int row = -1;
-    if (real) row = PART ? a.order[at] : at;
+    if (real) row = FORM == kPrefix ? a.order[at] : at;
     real = real && row >= 0 && row < a.n_rows;
     const int rc = real ? row : 0;
     // the walk, and lim, the last key the pair sees
     const int cap = a.max_pages << a.shift;
     Walk k;
     int lim, begin = 0;
-    k.own_t = a.tables + (int64_t)tile.x * a.max_pages;
+    k.own_t = a.tables + (int64_t)who * a.max_pages;
     k.pre_t = k.own_t;
     k.fresh0 = INT32_MAX;
     k.fresh_row = 0;
-    if (PART) {
+    if (FORM == kPrefix) {
         k.plen = 0;
         prefix_of(a, rc, lim);
         lim = real ? lim - 1 : -1;
         // this workgroup's keys, the same for all pairs of the tile
-        const int keys = min(max(tile.w, 0), cap);
+        keys = min(max(keys, 0), cap);
         const int used = min(a.n_shared, (keys + kMinPart - 1) / kMinPart);
         const int size = used > 0 ? ((keys + used - 1) / used + 31) / 32 * 32 : 0;
         begin = min((int)blockIdx.y * size, keys);
         k.end = min(begin + size, keys);
     } else {
-        const int pre = prefix_of(a, tile.x, k.plen);
+        const int pre = prefix_of(a, who, k.plen);
         if (pre >= 0) k.pre_t = a.tables + (int64_t)pre * a.max_pages;
         lim = real ? min(a.position[rc], k.plen + cap - 1) : -1;
-        k.end = min(tile.w, k.plen + cap);
-        if (a.k) {  // the stream's first new row and its position
-            k.fresh_row = min(max(a.row_start[tile.x], 0), first);
+        k.end = min(keys, k.plen + cap);
+        if (PROMPT && a.k) {  // the stream's first new row and its position
+            k.fresh_row = min(max(a.row_start[who], 0), first);
             k.fresh0 = max(a.position[min(first, a.n_rows - 1)] - (first - k.fresh_row), 0);
         }
         // with SPLIT, the pairs' last key ends the walk
-        if (SPLIT) {
+        if (PROMPT && SPLIT) {
             const int end_row = first + over_group(a, min(p0 + 15, pairs - 1));
             k.end = min(k.end, a.position[min(end_row, a.n_rows - 1)] + 1);
+        }
+        if (FORM == kOneRow) {  // a part of the row's keys: its own alone where tiles take the prefix
+            const int pos = a.position[first], stop = min(pos + 1, k.plen + cap);
+            begin = a.tiles ? min(k.plen, pos + 1) : 0;
+            const int L = max(stop - begin, 0);
+            const int used = min(max(a.n_own, 1), (L + a.min_part - 1) / a.min_part);
+            const int size = used > 0 ? ((L + used - 1) / used + 31) / 32 * 32 : 0;
+            begin = min(begin + (int)blockIdx.y * size, max(stop, 0));
+            k.end = min(begin + size, stop);
+            // the new row to its slot before it is read with the others
+            if (a.k && pos >= begin && pos < k.end) {
+                const int slot = a.slot[first];
+                const uint32_t home = cache_row(a, slot < 0 ? -1 : slot >> a.shift, kvh, slot);
+                if (home != kNoRow && tid < 16) {
+                    const int64_t x = first * a.ld_kv + kvh * kDim + 4 * tid;
+                    store4(const_cast<T*>(kc), home, 4 * tid, *reinterpret_cast<const f4*>(a.k + x));
+                    store4(const_cast<T*>(vc), home, 4 * tid, *reinterpret_cast<const f4*>(a.v + x));
+                }
+                __syncthreads();
+            }
         }
     }
     k.end = __builtin_amdgcn_readfirstlane(k.end);  // as the whole workgroup has it
     k.plen = __builtin_amdgcn_readfirstlane(k.plen);
     k.fresh0 = __builtin_amdgcn_readfirstlane(k.fresh0);
     k.fresh_row = __builtin_amdgcn_readfirstlane(k.fresh_row);
+    begin = __builtin_amdgcn_readfirstlane(begin);
     // a part in LDS: rows of eight 16-byte chunks, a row's in an order of its own
     // so that 16 rows' reads of one chunk fall in different banks
     const auto chunk_at = [&](char* base, int r, int ch) {
@@ -561,14 +636,14 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
     int next[kU];
     // a stage's loads, nothing of them used before they are stored: a chunk of
     // K and V each, the fp16 forms' new rows (fp32) in two
-    constexpr int kLoads = F16 && !PART ? 2 : 1;
+    constexpr int kLoads = F16 && PROMPT ? 2 : 1;
     u4 kr[kU][kLoads], vr[kU][kLoads];
     uint32_t none = 0, fresh = 0;  // rows that have no place, and new ones: a bit each
     // the tile's own new rows (with SPLIT, those that begin among its pairs) go to
     // their slots as they are staged: rows [own0, own1) of the call
     uint32_t to[kU];
-    const int own0 = PART || !a.k ? 0 : first + over_group(a, p0 + a.group - 1);
-    const int own1 = PART || !a.k ? 0 : min(first + min(SPLIT ? over_group(a, p0 + 15 + a.group) : count, count), a.n_rows);
+    const int own0 = !PROMPT || !a.k ? 0 : first + over_group(a, p0 + a.group - 1);
+    const int own1 = !PROMPT || !a.k ? 0 : min(first + min(SPLIT ? over_group(a, p0 + 15 + a.group) : count, count), a.n_rows);
     const auto look = [&](int j0) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) next[u] = entry_of(a, k, j0 + r0 + u * kStep);
@@ -579,7 +654,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int j = j0 + r0 + u * kStep, place = j < k.plen ? j : j - k.plen;
-            const bool own = !PART && j >= k.fresh0;
+            const bool own = PROMPT && j >= k.fresh0;
             const uint32_t row = cache_row(a, own ? next[u] >> a.shift : next[u], kvh, place);
             if (j >= k.end || row == kNoRow) none |= 1u << u;
             uint64_t from = ((uint64_t)(row == kNoRow ? 0 : row) << 6) + kPer * ch;
@@ -596,7 +671,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
             }
             kr[u][0] = *reinterpret_cast<const u4*>(static_cast<const T*>(ks) + from);
             vr[u][0] = *reinterpret_cast<const u4*>(static_cast<const T*>(vs) + from);
-            if constexpr (F16 && !PART) {
+            if constexpr (F16 && PROMPT) {
                 if (own) {
                     kr[u][1] = *reinterpret_cast<const u4*>(static_cast<const T*>(ks) + from + 8);
                     vr[u][1] = *reinterpret_cast<const u4*>(static_cast<const T*>(vs) + from + 8);
@@ -612,7 +687,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
                 if (none >> u & 1) {
                     if (ch == 0) atomicOr(&gone[slot][(r0 + u * kStep) >> 5], 1u << ((r0 + u * kStep) & 31));
                     kr[u][0] = vr[u][0] = u4{0, 0, 0, 0};
-                    if (F16 && !PART) kr[u][kLoads - 1] = vr[u][kLoads - 1] = u4{0, 0, 0, 0};
+                    if (F16 && PROMPT) kr[u][kLoads - 1] = vr[u][kLoads - 1] = u4{0, 0, 0, 0};
                 }
         }
         // 0 times every value: NaN once one is not finite
@@ -624,7 +699,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {  // K, V
                 u4 y = x ? vr[u][0] : kr[u][0];
-                if constexpr (F16 && !PART) {
+                if constexpr (F16 && PROMPT) {
                     if (fresh >> u & 1) {  // rounded as the cache will hold them
                         const f4 lo = __builtin_bit_cast(f4, y);
                         const f4 hi = __builtin_bit_cast(f4, x ? vr[u][1] : kr[u][1]);
@@ -633,7 +708,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
                                                       (_Float16)hi[2], (_Float16)hi[3]});
                     }
                 }
-                if (!PART && to[u] != kNoRow)
+                if (PROMPT && to[u] != kNoRow)
                     *reinterpret_cast<u4*>(const_cast<T*>(x ? vc : kc) + ((uint64_t)to[u] << 6) + kPer * ch) = y;
                 if constexpr (F16) {
                     if (x) {
@@ -874,10 +949,11 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
     // lane (g, c): dimensions 4 c .. of pair i
     const auto finish = [&](int i, float pm, float ps, const f4& po) {
         const int ri = __shfl(real ? row : a.n_rows, i), hi = __shfl(h, i);
-        if (PART) {
+        if (FORM == kPrefix || (FORM == kOneRow && a.n_own > 0)) {
             if (ri >= a.n_rows) return;
             constexpr float kDown = F16 ? 1.0f / 16384.0f : 1.0f;
-            const int64_t to = ((int64_t)(a.n_own + blockIdx.y) * a.n_rows + ri) * a.n_head + hi;
+            const int part = (FORM == kPrefix ? a.n_own : 0) + blockIdx.y;
+            const int64_t to = ((int64_t)part * a.n_rows + ri) * a.n_head + hi;
             if (c == 0) a.part_ms[to] = float2{pm, __fmul_rn(ps, kDown)};
             *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * c) = po * kDown;
         } else {
@@ -916,20 +992,27 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
 // How a call's keys are cut: parts of a row's own (0: whole rows, stored by
 // the workgroup itself) and of a prefix.
 struct Cut {
-    int own, shared;
+    int own, shared, min_part;
 };
+
+constexpr int64_t kWaveUnits = 2048;
+// Query heads to a key head from which an fp16 step runs on the matrix cores.
+constexpr int kMatrixGroup = 3;
 
 int head_chunk(int group) { return group >= 3 ? 4 : group; }
 
 Cut cut_of(const cbx_kv_attn& a) {
-    Cut c{0, 0};
+    Cut c{0, 0, kMinPart};
     if (a.rows->stream) return c;
     const int group = a.n_head / a.cache->n_head;
     const int chunks = (group + head_chunk(group) - 1) / head_chunk(group);
     const int64_t wgs = (int64_t)a.rows->n_rows * a.cache->n_head * chunks;
     const int64_t cap = (int64_t)a.streams->max_pages * a.cache->page_size;
-    const bool tiles = a.rows->tiles && a.streams->parent && a.streams->n_prefix > 0;
-    const int64_t longest = tiles || !a.streams->parent ? cap : 2 * cap;
+    const bool prefixes = a.streams->parent && a.streams->n_prefix > 0;
+    const bool tiles = a.rows->tiles && prefixes;
+    const int64_t longest = tiles || !prefixes ? cap : 2 * cap;
+    // parts worth a workgroup's start and end where there are enough of them
+    c.min_part = (int)std::min<int64_t>(std::max<int64_t>(wgs / 2, kMinPart), 512);
     int64_t own = (1024 + wgs - 1) / wgs;
     own = std::max(own, (longest + 1023) / 1024);
     own = std::min(own, std::min<int64_t>(64, (longest + kMinPart - 1) / kMinPart));
@@ -947,34 +1030,41 @@ Cut cut_of(const cbx_kv_attn& a) {
 template <class T>
 hipError_t launch_rows(const KvArgs& a, hipStream_t st) {
     const int G = head_chunk(a.group), chunks = (a.group + G - 1) / G;
-    const dim3 grid((unsigned)a.n_rows * a.n_kv * chunks, (unsigned)max(a.n_own, 1));
-    const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(64 * kRowWaves), 0, st, a);
-        return hipGetLastError();
-    };
-    return G == 1 ? go(kv_rows<T, 1>) : G == 2 ? go(kv_rows<T, 2>) : go(kv_rows<T, 4>);
-}
-
-template <class T>
-hipError_t launch_tiles(const KvArgs& a, bool part, hipStream_t st) {
-    const int64_t waves = (int64_t)a.n_tiles * 4 * a.n_kv * (part ? a.n_shared : 1);
-    const bool split = waves < 2048;
-    const dim3 grid((unsigned)a.n_kv * a.n_tiles * (split ? 4 : 1),
-                    (unsigned)(part ? a.n_shared : 1));
+    // a wave per row and head where those are many: no barrier, four heads a workgroup
+    const int64_t units = (int64_t)a.n_rows * a.n_kv * chunks;
+    const bool wave = units >= kWaveUnits;
+    const dim3 grid((unsigned)(wave ? (units + 3) / 4 : units), (unsigned)max(a.n_own, 1));
     const auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
         return hipGetLastError();
     };
-    if (part) return split ? go(kv_tiles<T, true, true>) : go(kv_tiles<T, false, true>);
-    return split ? go(kv_tiles<T, true, false>) : go(kv_tiles<T, false, false>);
+    if (wave) return G == 1 ? go(kv_rows<T, 1, 1>) : G == 2 ? go(kv_rows<T, 2, 1>) : go(kv_rows<T, 4, 1>);
+    return G == 1 ? go(kv_rows<T, 1, 4>) : G == 2 ? go(kv_rows<T, 2, 4>) : go(kv_rows<T, 4, 4>);
+}
+
+template <class T>
+hipError_t launch_tiles(const KvArgs& a, int form, hipStream_t st) {
+    const int cuts = form == kPrompt ? 1 : form == kPrefix ? a.n_shared : max(a.n_own, 1);
+    const bool split = (int64_t)a.n_tiles * 4 * a.n_kv * cuts < 2048;
+    const int64_t units = form == kOneRow ? (int64_t)a.n_rows * ((a.group + 15) / 16)
+                                          : (int64_t)a.n_tiles * (split ? 4 : 1);
+    const dim3 grid((unsigned)(a.n_kv * units), (unsigned)cuts);
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+        return hipGetLastError();
+    };
+    if (form == kOneRow) return go(kv_tiles<T, true, kOneRow>);
+    if (form == kPrefix) return split ? go(kv_tiles<T, true, kPrefix>) : go(kv_tiles<T, false, kPrefix>);
+    return split ? go(kv_tiles<T, true, kPrompt>) : go(kv_tiles<T, false, kPrompt>);
 }
 
 template <class T>
 hipError_t launch(const KvArgs& a, bool step, hipStream_t st) {
     hipError_t e;
-    if (!step) return launch_tiles<T>(a, false, st);
-    if (a.n_shared && (e = launch_tiles<T>(a, true, st)) != hipSuccess) return e;
-    if ((e = launch_rows<T>(a, st)) != hipSuccess || !a.n_own) return e;
+    if (!step) return launch_tiles<T>(a, kPrompt, st);
+    if (a.n_shared && (e = launch_tiles<T>(a, kPrefix, st)) != hipSuccess) return e;
+    e = sizeof(T) == 2 && a.group >= kMatrixGroup ? launch_tiles<T>(a, kOneRow, st) : launch_rows<T>(a, st);
+    if (e != hipSuccess || !a.n_own) return e;
     const int64_t waves = (int64_t)a.n_rows * a.n_head;
     hipLaunchKernelGGL(kv_join, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a);
     return hipGetLastError();
@@ -1030,6 +1120,7 @@ hipError_t launch_kv_attend(const cbx_kv_attn& c, uint32_t* parts, float* inv, h
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + (n * 8 + 255) / 256 * 256);
     a.n_own = cut.own;
     a.n_shared = cut.shared;
+    a.min_part = cut.min_part;
     return p.type == CBX_KV_F32 ? launch<float>(a, !r.stream, st) : launch<_Float16>(a, !r.stream, st);
 }
 
