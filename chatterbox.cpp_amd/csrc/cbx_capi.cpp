@@ -631,8 +631,8 @@ int check_kv_attn(const char* fn, const cbx_kv_attn* a) {
         return fail(CBX_ERR_INVALID, "%s: tile_rows %d, %d wanted", fn, a->rows->tile_rows,
                     cbx_kv_tile_rows(a->n_head, c.n_head));
     // the launches' grids
-    if ((int64_t)a->rows->n_rows * a->n_head > 0x7fffffffLL ||
-        (a->rows->tiles && (int64_t)a->rows->n_tiles * c.n_head > 0x7fffffffLL))
+    if ((int64_t)a->rows->n_rows * a->n_head > 0xffffff ||
+        (a->rows->tiles && (int64_t)a->rows->n_tiles * c.n_head > 0xffffff))
         return fail(CBX_ERR_UNSUPPORTED, "%s: %d rows of %d heads", fn, a->rows->n_rows, a->n_head);
     return CBX_OK;
 }

@@ -142,17 +142,17 @@ struct Chunk<_Float16> {
 // and waves in a fixed order.  The row's new k and v come from its input row,
 // stored on the way.
 template <class T, int G, int W>
-__global__ __launch_bounds__(256) void kv_rows(KvArgs a) {
+__device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int part) {
     using C = Chunk<T>;
     constexpr int DPL = C::kN, LPK = kDim / DPL, KPI = 64 / LPK;  // dims a lane, lanes a key
     constexpr int kU = G > 2 || sizeof(T) == 2 ? 4 : 6;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int chunks = (a.group + G - 1) / G, per_row = a.n_kv * chunks;
-    const int64_t unit = W == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + w;
+    const int64_t unit = W == 4 ? block : (int64_t)block * 4 + w;
     if (unit >= (int64_t)a.n_rows * per_row) return;
     const int r = (int)(unit / per_row), y = (int)(unit % per_row);
     const int kvh = y / chunks, g0 = y % chunks * G, h0 = kvh * a.group + g0;
-    const int ng = min(G, a.group - g0), part = blockIdx.y;
+    const int ng = min(G, a.group - g0);
     const int sub = lane / LPK, d0 = lane % LPK * DPL;
     const int pos = a.position[r];
     const int slot = a.k ? a.slot[r] : -1;
@@ -509,7 +509,7 @@ __device__ __forceinline__ int entry_of(const KvArgs& a, const Walk& k, int j) {
 // vector units then spends its time on products).
 enum { kPrompt, kPrefix, kOneRow };
 template <class T, bool SPLIT, int FORM>
-__global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
+__device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32_t blocks, int cut) {
     constexpr bool F16 = sizeof(T) == 2, PROMPT = FORM == kPrompt;
     static_assert(SPLIT || FORM != kOneRow, "a row's heads are one wave's pairs");
     constexpr int kKeys = SPLIT ? 128 : 32;
@@ -531,13 +531,13 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
     __shared__ float join_m[4][16], join_s[4][16];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int g = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x % a.n_kv, unit = blockIdx.x / a.n_kv;
+    const int kvh = block % a.n_kv, unit = block / a.n_kv;
     const T* const kc = static_cast<const T*>(a.kc);
     const T* const vc = static_cast<const T*>(a.vc);
     const auto dead_rows = [&]() {  // rows behind the last give zeros
         if (!PROMPT) return;
         const int total = a.row_start[a.n_streams];
-        for (int64_t r = (int64_t)max(total, 0) + blockIdx.x; r < a.n_rows; r += gridDim.x)
+        for (int64_t r = (int64_t)max(total, 0) + block; r < a.n_rows; r += blocks)
             for (int h = w; h < a.n_head; h += 4) attn_store(a.o, (int)r, h, lane, 0.0f);
     };
     // the workgroup's rows: [first, first + count) of the call (of order, where
@@ -583,9 +583,9 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
         lim = real ? lim - 1 : -1;
         // this workgroup's keys, the same for all pairs of the tile
         keys = min(max(keys, 0), cap);
-        const int used = min(a.n_shared, (keys + kMinPart - 1) / kMinPart);
+        const int used = min(a.n_shared, (keys + 31) / 32);
         const int size = used > 0 ? ((keys + used - 1) / used + 31) / 32 * 32 : 0;
-        begin = min((int)blockIdx.y * size, keys);
+        begin = min(cut * size, keys);
         k.end = min(begin + size, keys);
     } else {
         const int pre = prefix_of(a, who, k.plen);
@@ -607,7 +607,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
             const int L = max(stop - begin, 0);
             const int used = min(max(a.n_own, 1), (L + a.min_part - 1) / a.min_part);
             const int size = used > 0 ? ((L + used - 1) / used + 31) / 32 * 32 : 0;
-            begin = min(begin + (int)blockIdx.y * size, max(stop, 0));
+            begin = min(begin + cut * size, max(stop, 0));
             k.end = min(begin + size, stop);
             // the new row to its slot before it is read with the others
             if (a.k && pos >= begin && pos < k.end) {
@@ -952,7 +952,7 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
         if (FORM == kPrefix || (FORM == kOneRow && a.n_own > 0)) {
             if (ri >= a.n_rows) return;
             constexpr float kDown = F16 ? 1.0f / 16384.0f : 1.0f;
-            const int part = (FORM == kPrefix ? a.n_own : 0) + blockIdx.y;
+            const int part = (FORM == kPrefix ? a.n_own : 0) + cut;
             const int64_t to = ((int64_t)part * a.n_rows + ri) * a.n_head + hi;
             if (c == 0) a.part_ms[to] = float2{pm, __fmul_rn(ps, kDown)};
             *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * c) = po * kDown;
@@ -987,6 +987,32 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
     dead_rows();
 }
 
+template <class T, int G, int W>
+__global__ __launch_bounds__(256) void kv_rows(KvArgs a) {
+    rows_of<T, G, W>(a, blockIdx.x, blockIdx.y);
+}
+
+template <class T, bool SPLIT, int FORM>
+__global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
+    tiles_of<T, SPLIT, FORM>(a, blockIdx.x, gridDim.x, blockIdx.y);
+}
+
+// A step with shared prefixes in one launch: first the workgroups of the
+// prefixes' tiles, then those of the rows' own keys (the vector units' or, MX,
+// the matrix cores' form): the tiles' products run beside the rows' reads.
+// us, two launches / one: 64 rows, a prefix of 377: ; 512 rows, one of 2001:
+template <class T, int G, int W, bool MX>
+__global__ __launch_bounds__(256, 3) void kv_shared(KvArgs a, uint32_t tile_blocks, uint32_t row_blocks) {
+    if (blockIdx.x < tile_blocks) {
+        const uint32_t n = tile_blocks / a.n_shared;
+        tiles_of<T, false, kPrefix>(a, blockIdx.x % n, n, blockIdx.x / n);
+    } else {
+        const uint32_t b = blockIdx.x - tile_blocks;
+        if constexpr (MX) tiles_of<T, true, kOneRow>(a, b % row_blocks, row_blocks, b / row_blocks);
+        else rows_of<T, G, W>(a, b % row_blocks, b / row_blocks);
+    }
+}
+
 // ------------------------------------------------------------------ launches
 
 // How a call's keys are cut: parts of a row's own (0: whole rows, stored by
@@ -996,8 +1022,6 @@ struct Cut {
 };
 
 constexpr int64_t kWaveUnits = 2048;
-// Query heads to a key head from which an fp16 step runs on the matrix cores.
-constexpr int kMatrixGroup = 3;
 
 int head_chunk(int group) { return group >= 3 ? 4 : group; }
 
@@ -1018,7 +1042,7 @@ Cut cut_of(const cbx_kv_attn& a) {
     own = std::min(own, std::min<int64_t>(64, (longest + kMinPart - 1) / kMinPart));
     if (tiles) {
         const int64_t t = (int64_t)a.rows->n_tiles * a.cache->n_head;
-        const int64_t most = std::min<int64_t>(32, (cap + kMinPart - 1) / kMinPart);
+        const int64_t most = std::min<int64_t>(32, (cap + 31) / 32);
         c.shared = (int)std::min(std::max<int64_t>((768 + t / 2) / t, 1), most);
         c.own = (int)own;
     } else {
@@ -1027,43 +1051,49 @@ Cut cut_of(const cbx_kv_attn& a) {
     return c;
 }
 
+// The step form: the rows' own keys, behind the prefixes' tiles where there are any.
 template <class T>
-hipError_t launch_rows(const KvArgs& a, hipStream_t st) {
+hipError_t launch_step(const KvArgs& a, hipStream_t st) {
     const int G = head_chunk(a.group), chunks = (a.group + G - 1) / G;
+    const bool matrix = sizeof(T) == 2 && a.group >= 3;
     // a wave per row and head where those are many: no barrier, four heads a workgroup
-    const int64_t units = (int64_t)a.n_rows * a.n_kv * chunks;
-    const bool wave = units >= kWaveUnits;
-    const dim3 grid((unsigned)(wave ? (units + 3) / 4 : units), (unsigned)max(a.n_own, 1));
-    const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
+    const int64_t units = (int64_t)a.n_rows * a.n_kv * (matrix ? (a.group + 15) / 16 : chunks);
+    const bool wave = !matrix && units >= kWaveUnits;
+    const unsigned blocks = (unsigned)(wave ? (units + 3) / 4 : units), cuts = (unsigned)max(a.n_own, 1);
+    const unsigned tiles = (unsigned)a.n_kv * a.n_tiles * a.n_shared;
+    const auto go = [&](auto rows, auto both) {
+        if (a.n_shared)
+            hipLaunchKernelGGL(both, dim3(tiles + blocks * cuts), dim3(256), 0, st, a, tiles, blocks);
+        else
+            hipLaunchKernelGGL(rows, dim3(blocks, cuts), dim3(256), 0, st, a);
         return hipGetLastError();
     };
-    if (wave) return G == 1 ? go(kv_rows<T, 1, 1>) : G == 2 ? go(kv_rows<T, 2, 1>) : go(kv_rows<T, 4, 1>);
-    return G == 1 ? go(kv_rows<T, 1, 4>) : G == 2 ? go(kv_rows<T, 2, 4>) : go(kv_rows<T, 4, 4>);
+    if (G == 1)
+        return wave ? go(kv_rows<T, 1, 1>, kv_shared<T, 1, 1, false>)
+                    : go(kv_rows<T, 1, 4>, kv_shared<T, 1, 4, false>);
+    if (G == 2)
+        return wave ? go(kv_rows<T, 2, 1>, kv_shared<T, 2, 1, false>)
+                    : go(kv_rows<T, 2, 4>, kv_shared<T, 2, 4, false>);
+    if constexpr (sizeof(T) == 2)
+        return go(kv_tiles<T, true, kOneRow>, kv_shared<T, 1, 4, true>);
+    else
+        return wave ? go(kv_rows<T, 4, 1>, kv_shared<T, 4, 1, false>)
+                    : go(kv_rows<T, 4, 4>, kv_shared<T, 4, 4, false>);
 }
 
 template <class T>
-hipError_t launch_tiles(const KvArgs& a, int form, hipStream_t st) {
-    const int cuts = form == kPrompt ? 1 : form == kPrefix ? a.n_shared : max(a.n_own, 1);
-    const bool split = (int64_t)a.n_tiles * 4 * a.n_kv * cuts < 2048;
-    const int64_t units = form == kOneRow ? (int64_t)a.n_rows * ((a.group + 15) / 16)
-                                          : (int64_t)a.n_tiles * (split ? 4 : 1);
-    const dim3 grid((unsigned)(a.n_kv * units), (unsigned)cuts);
-    const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
-        return hipGetLastError();
-    };
-    if (form == kOneRow) return go(kv_tiles<T, true, kOneRow>);
-    if (form == kPrefix) return split ? go(kv_tiles<T, true, kPrefix>) : go(kv_tiles<T, false, kPrefix>);
-    return split ? go(kv_tiles<T, true, kPrompt>) : go(kv_tiles<T, false, kPrompt>);
+hipError_t launch_prompt(const KvArgs& a, hipStream_t st) {
+    const bool split = (int64_t)a.n_tiles * 4 * a.n_kv < 2048;
+    const dim3 grid((unsigned)a.n_kv * a.n_tiles * (split ? 4 : 1));
+    if (split) hipLaunchKernelGGL((kv_tiles<T, true, kPrompt>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv_tiles<T, false, kPrompt>), grid, dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 template <class T>
 hipError_t launch(const KvArgs& a, bool step, hipStream_t st) {
-    hipError_t e;
-    if (!step) return launch_tiles<T>(a, kPrompt, st);
-    if (a.n_shared && (e = launch_tiles<T>(a, kPrefix, st)) != hipSuccess) return e;
-    e = sizeof(T) == 2 && a.group >= kMatrixGroup ? launch_tiles<T>(a, kOneRow, st) : launch_rows<T>(a, st);
+    if (!step) return launch_prompt<T>(a, st);
+    const hipError_t e = launch_step<T>(a, st);
     if (e != hipSuccess || !a.n_own) return e;
     const int64_t waves = (int64_t)a.n_rows * a.n_head;
     hipLaunchKernelGGL(kv_join, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, st, a);
