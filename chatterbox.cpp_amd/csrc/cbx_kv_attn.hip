@@ -4,19 +4,20 @@
 //
 // A row's positions [0, n) are its prefix's [0, plen), in the prefix's pages,
 // then its own, in its own pages from their first place on.  The softmax is
-// taken in one pass: over any set of keys, (m, s, o) = (max x, sum e^(x - m),
-// sum e^(x - m) v), and two sets' join as
-//   m = max(m1, m2), s = s1 e^(m1 - m) + s2 e^(m2 - m), o alike; out = o / s,
+// taken in one pass, e^x as 2^(x log2 e): over any set of keys, with a whole
+// number r >= max x log2 e, (r, s, o) = (r, sum w, sum w v), w = 2^(x log2 e - r),
+// and two sets join as
+//   r = max(r1, r2), s = s1 2^(r1 - r) + s2 2^(r2 - r), o alike; out = o / s,
 // so keys may be cut anywhere: over lanes, waves, workgroups, and into a
-// prefix's part computed once for many rows and each row's own.
+// prefix's part computed once for many rows and each row's own.  r whole: every
+// rescaling is by a power of two, and x log2 e - r one fused operation whose r
+// is the same for all keys of a set, so no rounding of the reference remains.
 //
 //  * kv_rows: the step form, one row a stream, on the vector units: what
 //    bounds it is reading each stream's keys and values.
 //  * kv_tiles: the prompt form, and the step form's shared prefixes: 16 (row,
 //    head) pairs a wave on the fp32 matrix cores.
 //  * kv_join: the parts of rows whose keys were cut over workgroups.
-// e^x as 2^(x log2 e): the difference x - m is formed first, so that the
-// product's rounding is relative to it.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -36,7 +37,12 @@ constexpr uint32_t kNoRow = ~0u;  // a key without a page
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(__fmul_rn(d, kLog2e)); }
+// 2^(from - to) for references: 0 from a set without keys (-inf).
+__device__ __forceinline__ float rescale(float from, float to) {
+    return from == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__fsub_rn(from, to));
+}
+// The reference of scores up to x (c2: the scores' unit in powers of two).
+__device__ __forceinline__ float reference(float x, float c2) { return __builtin_ceilf(__fmul_rn(x, c2)); }
 
 struct KvArgs {
     const void* kc;  // this layer's pages: [page][n_kv][position][64]
@@ -258,7 +264,7 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                float x[kU], bm = m[g];
+                float x[kU], bm = -INFINITY;
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
                     float t = 0.0f;
@@ -276,18 +282,19 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
                 }
 #pragma unroll
                 for (int u = 0; u < kU; ++u) bm = fmaxf(bm, x[u]);
-                // a key that is not there, or -inf while none is larger, has weight 0
-                const float base = bm == -INFINITY ? 0.0f : bm;
-                if (__ballot(bm > m[g])) {
-                    const float f = exp_of(__fsub_rn(m[g], base));  // 0 from -inf, 1 where it stays
+                const float nr = fmaxf(m[g], reference(bm, kLog2e));
+                if (__ballot(nr > m[g])) {
+                    const float f = rescale(m[g], nr);
                     s[g] = __fmul_rn(s[g], f);
 #pragma unroll
                     for (int d = 0; d < DPL; ++d) o[g][d] = __fmul_rn(o[g][d], f);
-                    m[g] = bm;
+                    m[g] = nr;
                 }
+                // a key that is not there, or -inf while none is larger, has weight 0
+                const float off = m[g] == -INFINITY ? 0.0f : -m[g];
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const float e = exp_of(__fsub_rn(x[u], base));
+                    const float e = __builtin_amdgcn_exp2f(__fmaf_rn(x[u], kLog2e, off));
                     s[g] = __fadd_rn(s[g], e);
 #pragma unroll
                     for (int d = 0; d < DPL; ++d) o[g][d] = __fmaf_rn(C::at(vv[u], d), e, o[g][d]);
@@ -303,8 +310,7 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
         for (int x = LPK; x < 64; x <<= 1) {
             const float mo = __shfl_xor(m[g], x), so = __shfl_xor(s[g], x);
             const float M = fmaxf(m[g], mo);
-            const float f = m[g] == -INFINITY ? 0.0f : exp_of(__fsub_rn(m[g], M));
-            const float fo = mo == -INFINITY ? 0.0f : exp_of(__fsub_rn(mo, M));
+            const float f = rescale(m[g], M), fo = rescale(mo, M);
             s[g] = __fadd_rn(__fmul_rn(s[g], f), __fmul_rn(so, fo));
 #pragma unroll
             for (int d = 0; d < DPL; ++d)
@@ -352,7 +358,7 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
             float st = 0.0f, ot = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float f = red_m[i][g] == -INFINITY ? 0.0f : exp_of(__fsub_rn(red_m[i][g], M));
+                const float f = rescale(red_m[i][g], M);
                 st = __fadd_rn(st, __fmul_rn(red_s[i][g], f));
                 ot = __fadd_rn(ot, __fmul_rn(red_o[i][g][lane], f));
             }
@@ -382,11 +388,11 @@ __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) bm = fmaxf(bm, __shfl_xor(bm, o));
         const float nm = fmaxf(M, bm);
-        const float keep = M == -INFINITY ? 0.0f : exp_of(__fsub_rn(M, nm));
+        const float keep = rescale(M, nm);
         st = __fmul_rn(st, keep);
         ot = __fmul_rn(ot, keep);
         M = nm;
-        const float f = ms.x == -INFINITY ? 0.0f : exp_of(__fsub_rn(ms.x, M));
+        const float f = rescale(ms.x, M);
         const float sf = __fmul_rn(ms.y, f);
         for (uint64_t left = __ballot(!(ms.y == 0.0f)); left; left &= left - 1) {
             const int i = (int)__builtin_ctzll(left);
@@ -432,6 +438,8 @@ struct Parts<float> {
             y = __fsub_rn(y, __builtin_bit_cast(float, v & 0xffff0000u));
         }
     }
+    __device__ static __forceinline__ void split_weights(float x, float y, uint32_t (&p)[3]) { split(x, y, p); }
+    static constexpr uint32_t kOnes = 0x3f803f80;
     __device__ static __forceinline__ f4 mfma(const u4& x, const u4& y, const f4& acc) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x),
                                                        __builtin_bit_cast(b8, y), acc, 0, 0, 0);
@@ -448,11 +456,33 @@ struct Parts<_Float16> {
         p[1] = __builtin_bit_cast(uint32_t, split_h2{(_Float16)__fsub_rn(x, (float)a),
                                                      (_Float16)__fsub_rn(y, (float)b)});
     }
+    // the weights': to 2^-20, both parts cut off instead of rounded (half the
+    // operations); what is cut leaves their sum too, which is taken of the parts
+    __device__ static __forceinline__ void split_weights(float x, float y, uint32_t (&p)[2]) {
+        p[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+        const split_h2 h = __builtin_bit_cast(split_h2, p[0]);
+        float one;  // opaque, for the mixed-precision form of x - hi
+        asm("v_mov_b32 %0, 1.0" : "=v"(one));
+        p[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(
+                                                __fmaf_rn(-(float)h[0], one, x), __fmaf_rn(-(float)h[1], one, y)));
+    }
+    static constexpr uint32_t kOnes = 0x3c003c00;
     __device__ static __forceinline__ f4 mfma(const u4& x, const u4& y, const f4& acc) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x),
                                                       __builtin_bit_cast(h8, y), acc, 0, 0, 0);
     }
 };
+
+// The largest of v over the four lanes of a 16-lane column (lane, lane ^ 16,
+// lane ^ 32, lane ^ 48).
+__device__ __forceinline__ float max_column(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const float m = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const uint32_t y = __builtin_bit_cast(uint32_t, m);
+    const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
 
 // Four keys of one dimension from rows of 16-bit values in LDS: of each 16
 // lanes, lane 4 r + q names 4 dimensions (quarter q of 16) of key r, and lane i
@@ -737,10 +767,10 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         if (F16) odd4 = (float)odd8[0] + (float)odd8[1];
         if (odd4 != odd4) odd[slot] = 1;
     };
-    // q, scaled: dimensions 32 ks + 8 g .. of pair c, in parts; a score is the
-    // matrix cores' times unit_of; c2: to powers of two
+    // q, scaled: dimensions 32 ks + 8 g .. of pair c, in parts; c2: a score as the
+    // matrix cores give it to powers of two
     u4 qp[2][P::kQ];
-    float unit_of = 1.0f, c2 = kLog2e;
+    float c2 = kLog2e;
     {
         const float* const qr = a.q + rc * a.ld_q + (real ? h : 0) * kDim;
         float x[2][8], mx = 0.0f;
@@ -757,10 +787,10 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
             }
         float sc = 1.0f;
         if (F16) {
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            split_scale(mx, sc, unit_of);
-            c2 = __fmul_rn(kLog2e, unit_of);
+            mx = max_column(mx);
+            float inv;
+            split_scale(mx, sc, inv);
+            c2 = __fmul_rn(kLog2e, inv);
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
@@ -776,7 +806,8 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     f4 o[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, s = 0.0f;  // m as the matrix cores give the scores
+    float ref = -INFINITY;
+    f4 sum = f4{0.0f, 0.0f, 0.0f, 0.0f};  // the first of it
     int last = lim, least = real ? lim : INT32_MAX;
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) {
@@ -822,39 +853,38 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                 for (int i = 0; i < 4; ++i)
                     if (!(see >> (16 * kt + i) & 1)) x[kt][i] = -INFINITY;
         }
-        float bm = -INFINITY;
+        float bm = fmaxf(x[0][0], x[1][0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bm = fmaxf(bm, fmaxf(x[0][i], x[1][i]));
-        bm = fmaxf(bm, __shfl_xor(bm, 16));
-        bm = fmaxf(bm, __shfl_xor(bm, 32));
-        if (__ballot(bm > m)) {
-            const float nm = fmaxf(m, bm);
-            const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, nm), c2));
-            s = __fmul_rn(s, f);
-            m = nm;
+        for (int i = 1; i < 4; ++i) bm = fmaxf(bm, fmaxf(x[0][i], x[1][i]));
+        const float nr = fmaxf(ref, reference(max_column(bm), c2));
+        if (__ballot(nr > ref)) {
+            const float f = rescale(ref, nr);
+            sum[0] = __fmul_rn(sum[0], f);
+            ref = nr;
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[dt][i] = __fmul_rn(o[dt][i], f);
         }
         // weights; unseen keys and scores of -inf have none
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float off = ref == -INFINITY ? 0.0f : __fsub_rn(kUp, ref);
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[kt][i] = __builtin_amdgcn_exp2f(__fmaf_rn(__fsub_rn(x[kt][i], base), c2, kUp));
-                s = __fadd_rn(s, x[kt][i]);
-            }
+            for (int i = 0; i < 4; ++i) x[kt][i] = __builtin_amdgcn_exp2f(__fmaf_rn(x[kt][i], c2, off));
         const bool plain = !(partial && __builtin_amdgcn_readfirstlane(odd[slot]));
         u4 wp[P::kQ];  // the weights' parts, the lane's eight keys
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             uint32_t y[P::kQ];
-            P::split(x[e >> 1][2 * (e & 1)], x[e >> 1][2 * (e & 1) + 1], y);
+            P::split_weights(x[e >> 1][2 * (e & 1)], x[e >> 1][2 * (e & 1) + 1], y);
 #pragma unroll
             for (int i = 0; i < P::kQ; ++i) wp[i][e] = y[i];
         }
+        // their sum, of the parts: every row of the product with ones
+#pragma unroll
+        for (int i = P::kQ - 1; i >= 0; --i)
+            sum = P::mfma(u4{P::kOnes, P::kOnes, P::kOnes, P::kOnes}, wp[i], sum);
         const auto value = [&](int dt, int i) {  // part i of dimension 16 dt + c of the lane's keys
             u4 y;
 #pragma unroll
@@ -933,8 +963,6 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         if (more) store(kBufs == 2 ? (t + 1) & 1 : 0, (t + 1) % 3);
         __syncthreads();
     }
-    s = __fadd_rn(s, __shfl_xor(s, 16));  // the pair's sum over its four lanes
-    s = __fadd_rn(s, __shfl_xor(s, 32));
     // through LDS into rows: [16 w + pair][dimension]
     float* const os = reinterpret_cast<float*>(lds) + 16 * w * kPad;
 #pragma unroll
@@ -942,8 +970,8 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         *reinterpret_cast<f4*>(os + c * kPad + 16 * i + 4 * g) = o[i];
     }
     if (g == 0) {
-        join_m[w][c] = __fmul_rn(m, unit_of);
-        join_s[w][c] = s;
+        join_m[w][c] = ref;
+        join_s[w][c] = sum[0];
     }
     __syncthreads();
     // lane (g, c): dimensions 4 c .. of pair i
@@ -976,7 +1004,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         f4 ot = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-            const float mx = join_m[x][i], f = mx == -INFINITY ? 0.0f : exp_of(__fsub_rn(mx, M));
+            const float f = rescale(join_m[x][i], M);
             st = __fadd_rn(st, __fmul_rn(join_s[x][i], f));
             const f4 ov = *reinterpret_cast<const f4*>(reinterpret_cast<float*>(lds) + (16 * x + i) * kPad + 4 * c);
 #pragma unroll
