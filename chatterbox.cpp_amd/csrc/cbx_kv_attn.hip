@@ -675,12 +675,40 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     const int own0 = !PROMPT || !a.k ? 0 : first + over_group(a, p0 + a.group - 1);
     const int own1 = !PROMPT || !a.k ? 0 : min(first + min(SPLIT ? over_group(a, p0 + 15 + a.group) : count, count), a.n_rows);
     const auto look = [&](int j0) {
+        if (PROMPT && j0 >= k.fresh0) {  // the call's own rows alone: their slots
+            const int r = k.fresh_row + (j0 - k.fresh0) + r0;
 #pragma unroll
-        for (int u = 0; u < kU; ++u) next[u] = entry_of(a, k, j0 + r0 + u * kStep);
+            for (int u = 0; u < kU; ++u) next[u] = a.slot[min(r + u * kStep, a.n_rows - 1)];
+        } else {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) next[u] = entry_of(a, k, j0 + r0 + u * kStep);
+        }
     };
     // the stage from j0 on, its entries in next
     const auto load = [&](int j0) {
         none = fresh = 0;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) to[u] = kNoRow;
+        if (PROMPT && j0 >= k.fresh0) {
+            const int rf = k.fresh_row + (j0 - k.fresh0);  // the stage's first row
+            const bool mine = rf < own1 && rf + kKeys > own0;
+            fresh = (1u << kU) - 1;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int r = min(rf + r0 + u * kStep, a.n_rows - 1);
+                if (j0 + r0 + u * kStep >= k.end || (uint32_t)next[u] >= (uint32_t)a.n_pages << a.shift)
+                    none |= 1u << u;
+                else if (mine && r >= own0 && r < own1)
+                    to[u] = cache_row(a, next[u] >> a.shift, kvh, next[u]);
+                const uint64_t from = (uint64_t)(uint32_t)r * (uint32_t)a.ld_kv + (kvh * kDim + kPer * ch);
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    kr[u][i] = *reinterpret_cast<const u4*>(a.k + from + 4 * i);
+                    vr[u][i] = *reinterpret_cast<const u4*>(a.v + from + 4 * i);
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
             const int j = j0 + r0 + u * kStep, place = j < k.plen ? j : j - k.plen;
@@ -689,7 +717,6 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
             if (j >= k.end || row == kNoRow) none |= 1u << u;
             uint64_t from = ((uint64_t)(row == kNoRow ? 0 : row) << 6) + kPer * ch;
             const void *ks = kc, *vs = vc;
-            to[u] = kNoRow;
             if (own) {
                 fresh |= 1u << u;
                 const int r = min(k.fresh_row + (j - k.fresh0), a.n_rows - 1);
@@ -802,7 +829,9 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                 for (int i = 0; i < P::kQ; ++i) qp[ks][i][e] = y[i];
             }
     }
-    constexpr float kUp = F16 ? 14.0f : 0.0f;  // the weights' scale, a power of two
+    // the weights' scale, a power of two, and how far one may pass it: with fp16
+    // parts by 2 (below 65504)
+    constexpr float kUp = F16 ? 14.0f : 0.0f, kSlack = F16 ? 1.0f : 16.0f;
     f4 o[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -853,25 +882,38 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                 for (int i = 0; i < 4; ++i)
                     if (!(see >> (16 * kt + i) & 1)) x[kt][i] = -INFINITY;
         }
-        float bm = fmaxf(x[0][0], x[1][0]);
+        // exponents by the pair's reference (by 0 before it has one); a larger one
+        // than kSlack over it moves the reference up
+        const float off = ref == -INFINITY ? kUp : __fsub_rn(kUp, ref);
+        float top = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < 4; ++i) bm = fmaxf(bm, fmaxf(x[0][i], x[1][i]));
-        const float nr = fmaxf(ref, reference(max_column(bm), c2));
-        if (__ballot(nr > ref)) {
-            const float f = rescale(ref, nr);
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[kt][i] = __fmaf_rn(x[kt][i], c2, off);
+                top = fmaxf(top, x[kt][i]);
+            }
+        top = max_column(top);
+        const bool move = ref == -INFINITY ? top > -INFINITY : top > kUp + kSlack;
+        if (__ballot(move)) {
+            const float by = move ? __builtin_ceilf(__fsub_rn(top, kUp)) : 0.0f;
+            const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by);
+            ref = !move ? ref : ref == -INFINITY ? by : __fadd_rn(ref, by);
             sum[0] = __fmul_rn(sum[0], f);
-            ref = nr;
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[dt][i] = __fmul_rn(o[dt][i], f);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[kt][i] = __fsub_rn(x[kt][i], by);
         }
         // weights; unseen keys and scores of -inf have none
-        const float off = ref == -INFINITY ? 0.0f : __fsub_rn(kUp, ref);
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[kt][i] = __builtin_amdgcn_exp2f(__fmaf_rn(x[kt][i], c2, off));
+            for (int i = 0; i < 4; ++i) x[kt][i] = __builtin_amdgcn_exp2f(x[kt][i]);
         const bool plain = !(partial && __builtin_amdgcn_readfirstlane(odd[slot]));
         u4 wp[P::kQ];  // the weights' parts, the lane's eight keys
 #pragma unroll
