@@ -406,6 +406,9 @@ __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
 // ------------------------------------------------------------------ tiles
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+// addresses chosen among several are kept as ones of device memory
+typedef const __attribute__((address_space(1))) u4* global_u4;
+typedef const __attribute__((address_space(1))) int32_t* global_i32;
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
@@ -501,17 +504,6 @@ struct Walk {
     const int32_t* own_t;
     int plen, end, fresh0, fresh_row;
 };
-
-// The table entry that says where key j < end is (the new rows': their slot);
-// read without a branch, so that nothing waits for it before it is used.
-__device__ __forceinline__ int entry_of(const KvArgs& a, const Walk& k, int j) {
-    const int x = min(j, k.end - 1);
-    const bool theirs = x < k.plen;
-    const int place = theirs ? x : x - k.plen;
-    const int32_t* p = (theirs ? k.pre_t : k.own_t) + (place >> a.shift);
-    if (x >= k.fresh0) p = a.slot + min(k.fresh_row + (x - k.fresh0), a.n_rows - 1);
-    return *p;
-}
 
 // 16 (row, head) pairs of a tile a wave, on the matrix cores.  The keys and
 // values of a stage (kKeys of them) are loaded once for the workgroup, through
@@ -674,65 +666,86 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     uint32_t to[kU];
     const int own0 = !PROMPT || !a.k ? 0 : first + over_group(a, p0 + a.group - 1);
     const int own1 = !PROMPT || !a.k ? 0 : min(first + min(SPLIT ? over_group(a, p0 + 15 + a.group) : count, count), a.n_rows);
+    // the table entry that says where key j < end is (a new row's: its slot).  Here
+    // and in load the addresses may come by a branch, the loads themselves stand
+    // after it: a load on one side alone is waited for where the sides meet.
     const auto look = [&](int j0) {
-        if (PROMPT && j0 >= k.fresh0) {  // the call's own rows alone: their slots
+        const int32_t* from[kU];
+        if (PROMPT && j0 >= k.fresh0) {  // the call's own rows alone
             const int r = k.fresh_row + (j0 - k.fresh0) + r0;
 #pragma unroll
-            for (int u = 0; u < kU; ++u) next[u] = a.slot[min(r + u * kStep, a.n_rows - 1)];
+            for (int u = 0; u < kU; ++u) from[u] = a.slot + min(r + u * kStep, a.n_rows - 1);
         } else {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) next[u] = entry_of(a, k, j0 + r0 + u * kStep);
+            for (int u = 0; u < kU; ++u) {
+                const int x = min(j0 + r0 + u * kStep, k.end - 1);
+                const bool theirs = x < k.plen;
+                from[u] = (theirs ? k.pre_t : k.own_t) + ((theirs ? x : x - k.plen) >> a.shift);
+                if (PROMPT && x >= k.fresh0) from[u] = a.slot + min(k.fresh_row + (x - k.fresh0), a.n_rows - 1);
+            }
         }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) next[u] = *(global_i32)from[u];
     };
     // the stage from j0 on, its entries in next
+    const uint32_t places = (uint32_t)a.n_pages << a.shift, in_page = (1u << a.shift) - 1;
     const auto load = [&](int j0) {
         none = fresh = 0;
-#pragma unroll
-        for (int u = 0; u < kU; ++u) to[u] = kNoRow;
+        const char *ks[kU], *vs[kU];
+        const int rf = k.fresh_row + (j0 - k.fresh0);  // the stage's first row, where all are new
         if (PROMPT && j0 >= k.fresh0) {
-            const int rf = k.fresh_row + (j0 - k.fresh0);  // the stage's first row
-            const bool mine = rf < own1 && rf + kKeys > own0;
             fresh = (1u << kU) - 1;
 #pragma unroll
             for (int u = 0; u < kU; ++u) {
                 const int r = min(rf + r0 + u * kStep, a.n_rows - 1);
-                if (j0 + r0 + u * kStep >= k.end || (uint32_t)next[u] >= (uint32_t)a.n_pages << a.shift)
-                    none |= 1u << u;
-                else if (mine && r >= own0 && r < own1)
-                    to[u] = cache_row(a, next[u] >> a.shift, kvh, next[u]);
+                none |= (uint32_t)(j0 + r0 + u * kStep >= k.end || (uint32_t)next[u] >= places) << u;
                 const uint64_t from = (uint64_t)(uint32_t)r * (uint32_t)a.ld_kv + (kvh * kDim + kPer * ch);
+                ks[u] = reinterpret_cast<const char*>(a.k + from);
+                vs[u] = reinterpret_cast<const char*>(a.v + from);
+                to[u] = kNoRow;
+            }
+            if (rf < own1 && rf + kKeys > own0) {
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    kr[u][i] = *reinterpret_cast<const u4*>(a.k + from + 4 * i);
-                    vr[u][i] = *reinterpret_cast<const u4*>(a.v + from + 4 * i);
+                for (int u = 0; u < kU; ++u) {
+                    const int r = rf + r0 + u * kStep;
+                    const uint32_t row = (((uint32_t)(next[u] >> a.shift) * (uint32_t)a.n_kv + (uint32_t)kvh)
+                                          << a.shift) + ((uint32_t)next[u] & in_page);
+                    to[u] = !(none >> u & 1) && r >= own0 && r < own1 ? row : kNoRow;
                 }
             }
-            return;
+        } else {
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int j = j0 + r0 + u * kStep;
+                const bool own = PROMPT && j >= k.fresh0;
+                const int page = own ? next[u] >> a.shift : next[u];
+                const int off = own ? next[u] : j < k.plen ? j : j - k.plen;
+                const bool there = (uint32_t)page < (uint32_t)a.n_pages;
+                const uint32_t row = there ? (((uint32_t)page * (uint32_t)a.n_kv + (uint32_t)kvh) << a.shift) +
+                                                 ((uint32_t)off & in_page) : 0;
+                none |= (uint32_t)(j >= k.end || !there) << u;
+                const uint64_t from = ((uint64_t)row << 6) + kPer * ch;
+                ks[u] = reinterpret_cast<const char*>(kc + from);
+                vs[u] = reinterpret_cast<const char*>(vc + from);
+                to[u] = kNoRow;
+                if (PROMPT) {
+                    fresh |= (uint32_t)own << u;
+                    const int r = min(k.fresh_row + (j - k.fresh0), a.n_rows - 1);
+                    const uint64_t x = (uint64_t)(uint32_t)r * (uint32_t)a.ld_kv + (kvh * kDim + kPer * ch);
+                    ks[u] = own ? reinterpret_cast<const char*>(a.k + x) : ks[u];
+                    vs[u] = own ? reinterpret_cast<const char*>(a.v + x) : vs[u];
+                    to[u] = own && !(none >> u & 1) && r >= own0 && r < own1 ? row : kNoRow;
+                }
+            }
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int j = j0 + r0 + u * kStep, place = j < k.plen ? j : j - k.plen;
-            const bool own = PROMPT && j >= k.fresh0;
-            const uint32_t row = cache_row(a, own ? next[u] >> a.shift : next[u], kvh, place);
-            if (j >= k.end || row == kNoRow) none |= 1u << u;
-            uint64_t from = ((uint64_t)(row == kNoRow ? 0 : row) << 6) + kPer * ch;
-            const void *ks = kc, *vs = vc;
-            if (own) {
-                fresh |= 1u << u;
-                const int r = min(k.fresh_row + (j - k.fresh0), a.n_rows - 1);
-                if (j < k.end && r >= own0 && r < own1) to[u] = row;
-                from = (uint64_t)r * (uint32_t)a.ld_kv + kvh * kDim + kPer * ch;
-                ks = a.k;
-                vs = a.v;
-                if (F16) from *= 2;  // in fp16 units
-            }
-            kr[u][0] = *reinterpret_cast<const u4*>(static_cast<const T*>(ks) + from);
-            vr[u][0] = *reinterpret_cast<const u4*>(static_cast<const T*>(vs) + from);
-            if constexpr (F16 && PROMPT) {
-                if (own) {
-                    kr[u][1] = *reinterpret_cast<const u4*>(static_cast<const T*>(ks) + from + 8);
-                    vr[u][1] = *reinterpret_cast<const u4*>(static_cast<const T*>(vs) + from + 8);
-                }
+            kr[u][0] = *(global_u4)(ks[u]);
+            vr[u][0] = *(global_u4)(vs[u]);
+            if (kLoads == 2) {  // a new row's other half; a cached chunk again
+                const int more = fresh >> u & 1 ? 16 : 0;
+                kr[u][kLoads - 1] = *(global_u4)(ks[u] + more);
+                vr[u][kLoads - 1] = *(global_u4)(vs[u] + more);
             }
         }
     };
