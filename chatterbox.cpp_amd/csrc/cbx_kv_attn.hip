@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cbx_attn_out.h"
 #include "cbx_internal.h"
@@ -481,10 +482,13 @@ struct Parts<_Float16> {
 __device__ __forceinline__ float max_column(float v) {
     const uint32_t x = __builtin_bit_cast(uint32_t, v);
     const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    const float m = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    // the median with infinity: a maximum without a maximum's quieting of its operands
+    const float m = __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, (uint32_t)a[0]),
+                                            __builtin_bit_cast(float, (uint32_t)a[1]), INFINITY);
     const uint32_t y = __builtin_bit_cast(uint32_t, m);
     const auto b = __builtin_amdgcn_permlane32_swap(y, y, false, false);
-    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+    return __builtin_amdgcn_fmed3f(__builtin_bit_cast(float, (uint32_t)b[0]),
+                                   __builtin_bit_cast(float, (uint32_t)b[1]), INFINITY);
 }
 
 // Four keys of one dimension from rows of 16-bit values in LDS: of each 16
@@ -539,6 +543,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     constexpr int kCh = kDim * sizeof(T) / 16;       // 16-byte chunks of a row in memory
     constexpr int kStep = 256 / kCh;                 // rows that the workgroup loads at a time
     constexpr int kU = kKeys / kStep;               // rows a thread loads of a stage
+    static_assert(kStep % 16 == 0, "a thread's rows have one order of chunks");
     constexpr int kPer = 16 / sizeof(T);             // values of a chunk
     constexpr int kPad = kDim + 4;                   // a pair's outputs in LDS
     constexpr int kPart = kKeys * kDim * 2, kStage = P::kKv * kPart;  // bytes: a part, K or V
@@ -572,7 +577,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         count = 1;
         keys = 0;
     } else {
-        const int4 tile = a.tiles[SPLIT ? unit / 4 : unit];
+        const int4 tile = a.tiles[PROMPT ? a.n_tiles - 1 - (SPLIT ? unit / 4 : unit) : unit];
         who = __builtin_amdgcn_readfirstlane(tile.x);
         first = min(max(__builtin_amdgcn_readfirstlane(tile.y), 0), a.n_rows);
         count = min(__builtin_amdgcn_readfirstlane(tile.z), a.tile_rows);
@@ -651,9 +656,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     begin = __builtin_amdgcn_readfirstlane(begin);
     // a part in LDS: rows of eight 16-byte chunks, a row's in an order of its own
     // so that 16 rows' reads of one chunk fall in different banks
-    const auto chunk_at = [&](char* base, int r, int ch) {
-        return base + (r * 8 + (ch ^ (r >> 1 & 7))) * 16;
-    };
+    const auto chunk_at = [](int r, int ch) { return (r * 8 + (ch ^ (r >> 1 & 7))) * 16; };
     const int ch = tid % kCh, r0 = tid / kCh;
     int next[kU];
     // a stage's loads, nothing of them used before they are stored: a chunk of
@@ -661,6 +664,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     constexpr int kLoads = F16 && PROMPT ? 2 : 1;
     u4 kr[kU][kLoads], vr[kU][kLoads];
     uint32_t none = 0, fresh = 0;  // rows that have no place, and new ones: a bit each
+    bool some_new = false;  // in the stage, and so for the workgroup
     // the tile's own new rows (with SPLIT, those that begin among its pairs) go to
     // their slots as they are staged: rows [own0, own1) of the call
     uint32_t to[kU];
@@ -693,6 +697,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         none = fresh = 0;
         const char *ks[kU], *vs[kU];
         const int rf = k.fresh_row + (j0 - k.fresh0);  // the stage's first row, where all are new
+        some_new = PROMPT && j0 + kKeys > k.fresh0;
         if (PROMPT && j0 >= k.fresh0) {
             fresh = (1u << kU) - 1;
 #pragma unroll
@@ -714,29 +719,34 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                 }
             }
         } else {
+            const auto places_of = [&](auto mixed) {
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int j = j0 + r0 + u * kStep;
-                const bool own = PROMPT && j >= k.fresh0;
-                const int page = own ? next[u] >> a.shift : next[u];
-                const int off = own ? next[u] : j < k.plen ? j : j - k.plen;
-                const bool there = (uint32_t)page < (uint32_t)a.n_pages;
-                const uint32_t row = there ? (((uint32_t)page * (uint32_t)a.n_kv + (uint32_t)kvh) << a.shift) +
-                                                 ((uint32_t)off & in_page) : 0;
-                none |= (uint32_t)(j >= k.end || !there) << u;
-                const uint64_t from = ((uint64_t)row << 6) + kPer * ch;
-                ks[u] = reinterpret_cast<const char*>(kc + from);
-                vs[u] = reinterpret_cast<const char*>(vc + from);
-                to[u] = kNoRow;
-                if (PROMPT) {
-                    fresh |= (uint32_t)own << u;
-                    const int r = min(k.fresh_row + (j - k.fresh0), a.n_rows - 1);
-                    const uint64_t x = (uint64_t)(uint32_t)r * (uint32_t)a.ld_kv + (kvh * kDim + kPer * ch);
-                    ks[u] = own ? reinterpret_cast<const char*>(a.k + x) : ks[u];
-                    vs[u] = own ? reinterpret_cast<const char*>(a.v + x) : vs[u];
-                    to[u] = own && !(none >> u & 1) && r >= own0 && r < own1 ? row : kNoRow;
+                for (int u = 0; u < kU; ++u) {
+                    const int j = j0 + r0 + u * kStep;
+                    const bool own = mixed && j >= k.fresh0;
+                    const int page = own ? next[u] >> a.shift : next[u];
+                    const int off = own ? next[u] : j < k.plen ? j : j - k.plen;
+                    const bool there = (uint32_t)page < (uint32_t)a.n_pages;
+                    uint32_t row = (((uint32_t)page * (uint32_t)a.n_kv + (uint32_t)kvh) << a.shift) +
+                                   ((uint32_t)off & in_page);
+                    row = there ? row : 0;
+                    none |= (uint32_t)(j >= k.end || !there) << u;
+                    const uint64_t from = (uint64_t)row << 6;
+                    ks[u] = reinterpret_cast<const char*>(kc + kPer * ch + from);
+                    vs[u] = reinterpret_cast<const char*>(vc + kPer * ch + from);
+                    to[u] = kNoRow;
+                    if (mixed) {
+                        fresh |= (uint32_t)own << u;
+                        const int r = min(k.fresh_row + (j - k.fresh0), a.n_rows - 1);
+                        const uint64_t x = (uint64_t)(uint32_t)r * (uint32_t)a.ld_kv + (kvh * kDim + kPer * ch);
+                        ks[u] = own ? reinterpret_cast<const char*>(a.k + x) : ks[u];
+                        vs[u] = own ? reinterpret_cast<const char*>(a.v + x) : vs[u];
+                        to[u] = own && !(none >> u & 1) && r >= own0 && r < own1 ? row : kNoRow;
+                    }
                 }
-            }
+            };
+            if (some_new) places_of(std::true_type());
+            else places_of(std::false_type());
         }
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
@@ -765,12 +775,11 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         split_h2 odd8 = split_h2{(_Float16)0.0f, (_Float16)0.0f};
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
-            const int r = r0 + u * kStep;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {  // K, V
                 u4 y = x ? vr[u][0] : kr[u][0];
                 if constexpr (F16 && PROMPT) {
-                    if (fresh >> u & 1) {  // rounded as the cache will hold them
+                    if (some_new && (fresh >> u & 1)) {  // rounded as the cache will hold them
                         const f4 lo = __builtin_bit_cast(f4, y);
                         const f4 hi = __builtin_bit_cast(f4, x ? vr[u][1] : kr[u][1]);
                         y = __builtin_bit_cast(u4, h8{(_Float16)lo[0], (_Float16)lo[1], (_Float16)lo[2],
@@ -778,7 +787,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                                                       (_Float16)hi[2], (_Float16)hi[3]});
                     }
                 }
-                if (PROMPT && to[u] != kNoRow)
+                if (PROMPT && some_new && to[u] != kNoRow)
                     *reinterpret_cast<u4*>(const_cast<T*>(x ? vc : kc) + ((uint64_t)to[u] << 6) + kPer * ch) = y;
                 if constexpr (F16) {
                     if (x) {
@@ -787,7 +796,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                         for (int i = 0; i < 4; ++i)
                             odd8 = __builtin_elementwise_fma(__builtin_bit_cast(split_h2, (uint32_t)y[i]), zero, odd8);
                     }
-                    *reinterpret_cast<u4*>(chunk_at(kb + x * kStage, r, ch)) = y;
+                    *reinterpret_cast<u4*>(kb + (chunk_at(r0, ch) + u * (kStep * 128) + x * kStage)) = y;
                 } else {
                     const f4 z = __builtin_bit_cast(f4, y);
                     if (x) {
@@ -799,8 +808,8 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                     P::split(z[2], z[3], hi);
 #pragma unroll
                     for (int i = 0; i < P::kKv; ++i)
-                        *reinterpret_cast<u2*>(chunk_at(kb + x * kStage + i * kPart, r, ch >> 1) +
-                                               8 * (ch & 1)) = u2{lo[i], hi[i]};
+                        *reinterpret_cast<u2*>(kb + (chunk_at(r0, ch >> 1) + 8 * (ch & 1) +
+                                                     u * (kStep * 128) + x * kStage + i * kPart)) = u2{lo[i], hi[i]};
                 }
             }
         }
@@ -848,7 +857,8 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     f4 o[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    float ref = -INFINITY;
+    // the exponents' offset and the exponent that moves the reference, kept with it
+    float ref = -INFINITY, off = kUp, bar = -INFINITY;
     f4 sum = f4{0.0f, 0.0f, 0.0f, 0.0f};  // the first of it
     int last = lim, least = real ? lim : INT32_MAX;
 #pragma unroll
@@ -859,10 +869,17 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     last = __builtin_amdgcn_readfirstlane(last);
     least = __builtin_amdgcn_readfirstlane(least);
 
+    // the lane's chunks of a buffer's first 16 rows: K's of key c, V's four
+    // dimensions of key 4 g + c / 4 (read_transposed)
+    int k_at[2], v_at[4];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) k_at[ks] = chunk_at(c, 4 * ks + g);
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) v_at[dt] = chunk_at(4 * g + (c >> 2), 2 * dt + (c >> 1 & 1)) + 8 * (c & 1);
+
     // 32 keys from j0 on: rows b .. of a buffer
     const auto compute = [&](int buf, int slot, int b, int j0) {
-        char* const kb = lds + 2 * buf * kStage;
-        char* const vb = kb + kStage;
+        const char* const kb = lds + 2 * buf * kStage + b * 128;  // 32 rows on, the order is the same
         const uint32_t miss = __builtin_amdgcn_readfirstlane(gone[slot][b >> 5]);
         f4 x[2] = {f4{0.0f, 0.0f, 0.0f, 0.0f}, f4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -872,8 +889,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int i = 0; i < P::kKv; ++i)
-                    y[kt][i] = *reinterpret_cast<const u4*>(
-                        chunk_at(kb + i * kPart, b + 16 * kt + c, 4 * ks + g));
+                    y[kt][i] = *reinterpret_cast<const u4*>(kb + k_at[ks] + (i * kPart + kt * 2048));
 #pragma unroll
             for (int i = 0; i < P::kProducts; ++i)
 #pragma unroll
@@ -897,7 +913,6 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         }
         // exponents by the pair's reference (by 0 before it has one); a larger one
         // than kSlack over it moves the reference up
-        const float off = ref == -INFINITY ? kUp : __fsub_rn(kUp, ref);
         float top = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -907,11 +922,15 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                 top = fmaxf(top, x[kt][i]);
             }
         top = max_column(top);
-        const bool move = ref == -INFINITY ? top > -INFINITY : top > kUp + kSlack;
+        const bool move = top > bar;
         if (__ballot(move)) {
             const float by = move ? __builtin_ceilf(__fsub_rn(top, kUp)) : 0.0f;
             const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by);
             ref = !move ? ref : ref == -INFINITY ? by : __fadd_rn(ref, by);
+            if (move) {
+                off = __fsub_rn(kUp, ref);
+                bar = kUp + kSlack;
+            }
             sum[0] = __fmul_rn(sum[0], f);
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt)
@@ -944,8 +963,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
             u4 y;
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
-                const u2 z = read_transposed(chunk_at(vb + i * kPart, b + 16 * kt + 4 * g + (c >> 2),
-                                                      2 * dt + (c >> 1 & 1)) + 8 * (c & 1));
+                const u2 z = read_transposed(kb + v_at[dt] + (kStage + i * kPart + kt * 2048));
                 y[2 * kt] = z[0];
                 y[2 * kt + 1] = z[1];
             }
