@@ -1094,7 +1094,7 @@ __global__ __launch_bounds__(256) void kv_rows(KvArgs a) {
 }
 
 template <class T, bool SPLIT, int FORM>
-__global__ __launch_bounds__(256, SPLIT ? 2 : 3) void kv_tiles(KvArgs a) {
+__global__ __launch_bounds__(256, SPLIT ? 2 : sizeof(T) == 2 ? 4 : 3) void kv_tiles(KvArgs a) {
     tiles_of<T, SPLIT, FORM>(a, blockIdx.x, gridDim.x, blockIdx.y);
 }
 
