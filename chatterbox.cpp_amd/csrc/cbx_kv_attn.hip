@@ -370,38 +370,66 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
 
 // ------------------------------------------------------------------ joins
 
-// One wave per row and head: the row's own parts and its prefix's.
+// One wave per row and head: the row's own parts and its prefix's, 64 at a
+// time: a lane each for maxima and sums, then each quarter of the wave every
+// fourth part's values, four to a lane and four loads in flight.
 __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (x >= (int64_t)a.n_rows * a.n_head) return;
     const int r = (int)(x / a.n_head), h = (int)(x % a.n_head);
     const int64_t rows = (int64_t)a.n_rows * a.n_head;
+    const int most = a.n_own + a.n_shared;
+    float2 ms = a.part_ms[min(lane, most - 1) * rows + x];
     int plen;
     prefix_of(a, r, plen);
     // parts of this row: none without a position
     const bool live = a.position[r] >= 0;
     const int n = live ? a.n_own + (plen > 0 ? a.n_shared : 0) : 0;
-    float M = -INFINITY, st = 0.0f, ot = 0.0f;
+    float M = -INFINITY, st = 0.0f;
+    f4 ot = f4{0.0f, 0.0f, 0.0f, 0.0f};
     for (int p0 = 0; p0 < n; p0 += 64) {
-        const float2 ms = p0 + lane < n ? a.part_ms[(p0 + lane) * rows + x] : float2{-INFINITY, 0.0f};
+        if (p0 > 0) ms = a.part_ms[min(p0 + lane, most - 1) * rows + x];
+        if (p0 + lane >= n) ms = float2{-INFINITY, 0.0f};
         float bm = ms.x;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) bm = fmaxf(bm, __shfl_xor(bm, o));
         const float nm = fmaxf(M, bm);
         const float keep = rescale(M, nm);
         st = __fmul_rn(st, keep);
-        ot = __fmul_rn(ot, keep);
+        ot *= keep;
         M = nm;
+        // a part that saw nothing has no values: they are not read into the sum
+        const uint64_t some = __ballot(!(ms.y == 0.0f));
         const float f = rescale(ms.x, M);
-        const float sf = __fmul_rn(ms.y, f);
-        for (uint64_t left = __ballot(!(ms.y == 0.0f)); left; left &= left - 1) {
-            const int i = (int)__builtin_ctzll(left);
-            st = __fadd_rn(st, __shfl(sf, i));
-            ot = __fadd_rn(ot, __fmul_rn(__shfl(f, i), a.part_o[((p0 + i) * rows + x) * kDim + lane]));
+        float sf = some >> lane & 1 ? __fmul_rn(ms.y, f) : 0.0f;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) sf = __fadd_rn(sf, __shfl_xor(sf, o));
+        st = __fadd_rn(st, sf);
+        const int last = some ? 64 - (int)__builtin_clzll(some) : 0;
+        for (int i0 = 0; i0 < last; i0 += 16) {
+            f4 y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                y[u] = *reinterpret_cast<const f4*>(
+                    a.part_o + ((p0 + min(i0 + 4 * u + g, last - 1)) * rows + x) * kDim + 4 * c);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = i0 + 4 * u + g;
+                const float fi = __shfl(f, i);
+                if (some >> i & 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ot[e] = __fadd_rn(ot[e], __fmul_rn(y[u][e], fi));
+                }
+            }
         }
     }
-    attn_store(a.o, r, h, lane, st == 0.0f ? 0.0f : __fdiv_rn(ot, st));
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ot[e] = __fadd_rn(ot[e], __shfl_xor(ot[e], o));
+    const float over = st == 0.0f ? 0.0f : __fdiv_rn(1.0f, st);
+    attn_store4(a.o, a.n_rows, g == 0 ? r : a.n_rows, h, c, ot * over);
 }
 
 // ------------------------------------------------------------------ tiles
