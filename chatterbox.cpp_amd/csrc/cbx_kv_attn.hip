@@ -638,7 +638,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         lim = real ? lim - 1 : -1;
         // this workgroup's keys, the same for all pairs of the tile
         keys = min(max(keys, 0), cap);
-        const int used = min(a.n_shared, (keys + 31) / 32);
+        const int used = min(a.n_shared, (keys + 63) / 64);
         const int size = used > 0 ? ((keys + used - 1) / used + 31) / 32 * 32 : 0;
         begin = min(cut * size, keys);
         k.end = min(begin + size, keys);
@@ -1171,8 +1171,8 @@ Cut cut_of(const cbx_kv_attn& a) {
     own = std::min(own, std::min<int64_t>(64, (longest + kMinPart - 1) / kMinPart));
     if (tiles) {
         const int64_t t = (int64_t)a.rows->n_tiles * a.cache->n_head;
-        const int64_t most = std::min<int64_t>(32, (cap + 31) / 32);
-        c.shared = (int)std::min(std::max<int64_t>((768 + t / 2) / t, 1), most);
+        const int64_t most = std::min<int64_t>(32, (cap + 63) / 64);
+        c.shared = (int)std::min(std::max<int64_t>((384 + t / 2) / t, 1), most);
         c.own = (int)own;
     } else {
         c.own = own > 1 ? (int)own : 0;
