@@ -15,9 +15,13 @@
 //
 //  * kv_rows: the step form, one row a stream, on the vector units: what
 //    bounds it is reading each stream's keys and values.
-//  * kv_tiles: the prompt form, and the step form's shared prefixes: 16 (row,
-//    head) pairs a wave on the fp32 matrix cores.
+//  * kv_tiles: the prompt form, and steps whose query heads share a key head:
+//    16 (row, head) pairs a wave on the 16-bit matrix cores.
+//  * kv_shared: steps with shared prefixes, a prefix's keys as tiles for all of
+//    its rows, the rows' own as in kv_rows or kv_tiles.
 //  * kv_join: the parts of rows whose keys were cut over workgroups.
+// Times are of the kernels on an MI355X, where a large copy moves 4.77 TB/s and
+// a large bf16 product runs at 1.15 PFLOP/s; 16 heads of 64 where not said.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -143,6 +147,7 @@ struct Chunk<_Float16> {
 
 // One part of one row's keys, for G of its key head's query heads, by W waves
 // (4: a workgroup; 1: the workgroup's waves take a head each, with no barrier).
+// Bound by the bytes: 64 rows of 129 to 383 fp32 keys 28.7 us, 4.7 TB/s.
 // LPK lanes to a key, 16 bytes of it each, kU keys per lane in flight; the page
 // ids of 64 pages are held by the wave's lanes, and handed over by an exchange.
 // Each lane group keeps a running (m, s, o) of its keys, joined over the groups
@@ -372,7 +377,8 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
 
 // One wave per row and head: the row's own parts and its prefix's, 64 at a
 // time: a lane each for maxima and sums, then each quarter of the wave every
-// fourth part's values, four to a lane and four loads in flight.
+// fourth part's values, four to a lane and four loads in flight (one part after
+// the other, 64 lanes a part: 6.6 us behind one row's parts where this takes 3.7).
 __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -557,10 +563,18 @@ struct Walk {
 // pair by pair with the unseen keys' V at 0.
 // SPLIT: the four waves take the same 16 pairs and 32 keys of a stage each,
 // joined through LDS (few rows); else each wave its own pairs and all keys.
-// FORM: the prompt form; the step form's prefixes, keys cut over blockIdx.y,
+// FORM: the prompt form; the step form's prefixes, keys cut over workgroups,
 // parts stored; or one row's heads of a key head against the row's keys, cut
 // likewise (where many query heads share a key head: the step form on the
 // vector units then spends its time on products).
+// Prompts of 4 x 4096 rows take fp32 965 us (142 TFLOP/s of the formula's, 850
+// of the parts'), fp16 530 (260, 585): the vector units' instructions (half the
+// time fp32, 60 % fp16) and the matrix cores' (43 %, 29 %) together.  64 prompts
+// of 129 to 383 rows fp32 129 us, 3.1 TB/s; 8 of 301 to 1501 fp16 behind 377 keys
+// 124.  Fewer instructions for a stage's addresses, all of K's reads before the
+// products, 8 waves a workgroup and two sets of pairs a wave were no faster or
+// slower; what was: stages loaded behind the choice of their addresses (fp16
+// 8 %), the longest tiles first (7 %), four workgroups a CU for fp16 (8 %).
 enum { kPrompt, kPrefix, kOneRow };
 template <class T, bool SPLIT, int FORM>
 __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32_t blocks, int cut) {
@@ -1116,9 +1130,9 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     dead_rows();
 }
 
-template <class T, int G, int W>
+template <class T, int G>
 __global__ __launch_bounds__(256) void kv_rows(KvArgs a) {
-    rows_of<T, G, W>(a, blockIdx.x, blockIdx.y);
+    rows_of<T, G, 4>(a, blockIdx.x, blockIdx.y);
 }
 
 template <class T, bool SPLIT, int FORM>
@@ -1129,7 +1143,10 @@ __global__ __launch_bounds__(256, SPLIT ? 2 : sizeof(T) == 2 ? 4 : 3) void kv_ti
 // A step with shared prefixes in one launch: first the workgroups of the
 // prefixes' tiles, then those of the rows' own keys (the vector units' or, MX,
 // the matrix cores' form): the tiles' products run beside the rows' reads.
-// us, two launches / one: 64 rows, a prefix of 377: ; 512 rows, one of 2001:
+// us, in two launches (prefixes + own) and in one: 64 rows behind a prefix of
+// 377 keys 15.5 + 9.4, 14.8; 512 rows of up to 64 behind one of 2001 48 + 25,
+// 54; 256 fp16 rows of up to 400 behind 8 of 250 to 500 11.6 + 23, 28.  The
+// rows have what the tiles leave of the LDS: three workgroups a CU for fp32.
 template <class T, int G, int W, bool MX>
 __global__ __launch_bounds__(256, 3) void kv_shared(KvArgs a, uint32_t tile_blocks, uint32_t row_blocks) {
     if (blockIdx.x < tile_blocks) {
@@ -1150,7 +1167,13 @@ struct Cut {
     int own, shared, min_part;
 };
 
-constexpr int64_t kWaveUnits = 2048;
+// Row heads from which rows beside prefixes' tiles get a wave each instead of a
+// workgroup.  us, a workgroup / a wave: fp32 rows of up to 300 behind a prefix
+// of 377, 64 of them 17.6 / 24.3, 128: 23.5 / 25.6, 256: 39.4 / 38.8; fp16 256
+// of them 30.7 / 26.1; 512 of 100 behind one of 2001: 142 / 110.  Without tiles
+// a workgroup each is as fast or faster at any number (256 fp32 rows of 129 to
+// 383: 100 / 107).
+constexpr int64_t kWaveUnits = 4096;
 
 int head_chunk(int group) { return group >= 3 ? 4 : group; }
 
@@ -1165,6 +1188,8 @@ Cut cut_of(const cbx_kv_attn& a) {
     const bool tiles = a.rows->tiles && prefixes;
     const int64_t longest = tiles || !prefixes ? cap : 2 * cap;
     // parts worth a workgroup's start and end where there are enough of them
+    // (256 fp16 rows of 64 to 4001 keys, four query heads a key head: 143 us
+    // with 64 keys a part, 94 with 512)
     c.min_part = (int)std::min<int64_t>(std::max<int64_t>(wgs / 2, kMinPart), 512);
     int64_t own = (1024 + wgs - 1) / wgs;
     own = std::max(own, (longest + 1023) / 1024);
@@ -1172,6 +1197,11 @@ Cut cut_of(const cbx_kv_attn& a) {
     if (tiles) {
         const int64_t t = (int64_t)a.rows->n_tiles * a.cache->n_head;
         const int64_t most = std::min<int64_t>(32, (cap + 63) / 64);
+        // prefixes' parts: enough workgroups that rows can run beside them, and
+        // not so many that all CUs are theirs first.  us with 768 / 384 / 256
+        // workgroups: 512 rows behind 2001 keys 58 / 54 / 71, 256 fp16 rows
+        // behind 8 prefixes 30.8 / 28.0 / 27.4; with parts of 32 / 64 keys at
+        // least 64 rows behind 377: 16.0 / 14.8
         c.shared = (int)std::min(std::max<int64_t>((384 + t / 2) / t, 1), most);
         c.own = (int)own;
     } else {
@@ -1184,35 +1214,40 @@ Cut cut_of(const cbx_kv_attn& a) {
 template <class T>
 hipError_t launch_step(const KvArgs& a, hipStream_t st) {
     const int G = head_chunk(a.group), chunks = (a.group + G - 1) / G;
+    // a key head's query heads are pairs of one tile.  us, vector units / matrix
+    // cores, 16 fp16 heads, rows of 1000 keys: 2 heads a key head, 64 rows 29.3 /
+    // 31.7; 4: 64 rows 25.9 / 21.6, 256 67.8 / 62.0; 8: 256 58.0 / 33.0
     const bool matrix = sizeof(T) == 2 && a.group >= 3;
-    // a wave per row and head where those are many: no barrier, four heads a workgroup
+    // beside prefixes' tiles a wave per row and head where those are many: four
+    // heads a workgroup, no barrier
     const int64_t units = (int64_t)a.n_rows * a.n_kv * (matrix ? (a.group + 15) / 16 : chunks);
-    const bool wave = !matrix && units >= kWaveUnits;
+    const bool wave = !matrix && a.n_shared && units >= kWaveUnits;
     const unsigned blocks = (unsigned)(wave ? (units + 3) / 4 : units), cuts = (unsigned)max(a.n_own, 1);
     const unsigned tiles = (unsigned)a.n_kv * a.n_tiles * a.n_shared;
-    const auto go = [&](auto rows, auto both) {
+    const auto go = [&](auto rows, auto both, auto waves) {
         if (a.n_shared)
-            hipLaunchKernelGGL(both, dim3(tiles + blocks * cuts), dim3(256), 0, st, a, tiles, blocks);
+            hipLaunchKernelGGL(wave ? waves : both, dim3(tiles + blocks * cuts), dim3(256), 0, st, a, tiles, blocks);
         else
             hipLaunchKernelGGL(rows, dim3(blocks, cuts), dim3(256), 0, st, a);
         return hipGetLastError();
     };
-    if (G == 1)
-        return wave ? go(kv_rows<T, 1, 1>, kv_shared<T, 1, 1, false>)
-                    : go(kv_rows<T, 1, 4>, kv_shared<T, 1, 4, false>);
-    if (G == 2)
-        return wave ? go(kv_rows<T, 2, 1>, kv_shared<T, 2, 1, false>)
-                    : go(kv_rows<T, 2, 4>, kv_shared<T, 2, 4, false>);
+    if (G == 1) return go(kv_rows<T, 1>, kv_shared<T, 1, 4, false>, kv_shared<T, 1, 1, false>);
+    if (G == 2) return go(kv_rows<T, 2>, kv_shared<T, 2, 4, false>, kv_shared<T, 2, 1, false>);
     if constexpr (sizeof(T) == 2)
-        return go(kv_tiles<T, true, kOneRow>, kv_shared<T, 1, 4, true>);
+        return go(kv_tiles<T, true, kOneRow>, kv_shared<T, 1, 4, true>, kv_shared<T, 1, 4, true>);
     else
-        return wave ? go(kv_rows<T, 4, 1>, kv_shared<T, 4, 1, false>)
-                    : go(kv_rows<T, 4, 4>, kv_shared<T, 4, 4, false>);
+        return go(kv_rows<T, 4>, kv_shared<T, 4, 4, false>, kv_shared<T, 4, 1, false>);
 }
 
 template <class T>
 hipError_t launch_prompt(const KvArgs& a, hipStream_t st) {
-    const bool split = (int64_t)a.n_tiles * 4 * a.n_kv < 2048;
+    // few tiles: four workgroups a tile, their waves the same pairs and other keys.
+    // Worth it while the workgroups (a.n_tiles counts a tile more per stream than
+    // there may be) are about the one or two a CU that fit: us, whole tiles /
+    // split, fp32: 1 x 256 rows 17.9 / 13.0, 1 x 384 24.6 / 21.0, 2 x 192 14.9 /
+    // 17.0, 4 x 256 20.3 / 40.6; fp16: 1 x 512 21.6 / 14.0, 2 x 256 13.7 / 11.4,
+    // 3 x 256 14.4 / 16.2
+    const bool split = (int64_t)a.n_tiles * 4 * a.n_kv <= (sizeof(T) == 4 ? 448 : 896);
     const dim3 grid((unsigned)a.n_kv * a.n_tiles * (split ? 4 : 1));
     if (split) hipLaunchKernelGGL((kv_tiles<T, true, kPrompt>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv_tiles<T, false, kPrompt>), grid, dim3(256), 0, st, a);
