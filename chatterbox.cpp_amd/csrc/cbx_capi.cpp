@@ -630,9 +630,9 @@ int check_kv_attn(const char* fn, const cbx_kv_attn* a) {
     if (a->rows->tiles && a->rows->tile_rows != cbx_kv_tile_rows(a->n_head, c.n_head))
         return fail(CBX_ERR_INVALID, "%s: tile_rows %d, %d wanted", fn, a->rows->tile_rows,
                     cbx_kv_tile_rows(a->n_head, c.n_head));
-    // the launches' grids
-    if ((int64_t)a->rows->n_rows * a->n_head > 0xffffff ||
-        (a->rows->tiles && (int64_t)a->rows->n_tiles * c.n_head > 0xffffff))
+    // the launches' grids: 2^24 workgroups of 256 at most
+    if ((int64_t)a->rows->n_rows * a->n_head +
+            (a->rows->tiles ? (int64_t)a->rows->n_tiles * c.n_head : 0) > cbx::kMaxKvGrid)
         return fail(CBX_ERR_UNSUPPORTED, "%s: %d rows of %d heads", fn, a->rows->n_rows, a->n_head);
     return CBX_OK;
 }
@@ -716,7 +716,7 @@ int t3_run(const char* fn, cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows
     if (!kv && (!cache->k || !cache->v || cache->n_ctx < 1 || cache->n_ctx > m->n_pos))
         return fail(CBX_ERR_INVALID, "%s: cache k/v NULL or n_ctx %d outside [1, n_pos]", fn,
                     cache->n_ctx);
-    if (cbx::t3_attn_lds(cache->n_ctx) + 2048 > s->lds_limit)
+    if (!kv && cbx::t3_attn_lds(cache->n_ctx) + 2048 > s->lds_limit)
         return fail(CBX_ERR_UNSUPPORTED, "%s: n_ctx %d: the attention's LDS exceeds the device's",
                     fn, cache->n_ctx);
     if (!positions || !hidden) return fail(CBX_ERR_INVALID, "%s: NULL positions or hidden", fn);

@@ -230,6 +230,8 @@ hipError_t launch_t3_step(const cbx_t3_model& m, int32_t n_rows, const int32_t* 
 // parts set: the output rows go there, split for the next product
 // (cbx_split.h), the scales to inv, instead of to a.out.
 constexpr int32_t kMaxKvStreams = 16384;
+// Workgroups of 256 that one grid dimension takes (2^32 - 1 threads).
+constexpr int64_t kMaxKvGrid = 0xffffff;
 hipError_t launch_kv_plan(const cbx_kv_plan& p, hipStream_t st);
 uint64_t kv_workspace_bytes(const cbx_kv_attn& a);
 hipError_t launch_kv_attend(const cbx_kv_attn& a, uint32_t* parts, float* inv, hipStream_t st);

@@ -451,8 +451,9 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 // fp32), two to a dword.
 //  * fp32 caches: three bf16 parts, each the leading 8 bits of what the ones
 //    before leave: x = h + m + l to the last bit wherever l is not subnormal,
-//    at any magnitude.  Of the nine products of two such values six are formed;
-//    m l, l m and l l are below 2^-23 of the whole.
+//    at any magnitude.  Of the nine products of two such values six are formed:
+//    |m| < 2^-7 |x| and |l| < 2^-15 |x|, so m l + l m + l l is below 2^-21 of the
+//    whole (and 2^-24 of it on average).
 //  * fp16 caches: keys and values as they are; queries and weights two fp16
 //    parts, x = hi + lo to 2^-22.
 // The fp32 matrix instructions run on the vector units' own multipliers, 32
@@ -1203,7 +1204,8 @@ Cut cut_of(const cbx_kv_attn& a) {
         // behind 8 prefixes 30.8 / 28.0 / 27.4; with parts of 32 / 64 keys at
         // least 64 rows behind 377: 16.0 / 14.8
         c.shared = (int)std::min(std::max<int64_t>((384 + t / 2) / t, 1), most);
-        c.own = (int)own;
+        // one grid holds both
+        c.own = (int)std::min(own, std::max<int64_t>((kMaxKvGrid - t * c.shared) / wgs, 1));
     } else {
         c.own = own > 1 ? (int)own : 0;
     }

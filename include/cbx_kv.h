@@ -47,9 +47,10 @@ typedef struct cbx_kv_cache {
 
 /* Streams of the pool.  Streams [0, n_prefix) are prefixes: filled like any
  * other, then shared.  A stream i >= n_prefix whose parent[i] is one of them
- * sees that prefix's first prefix_len[i] positions (any number it holds, also
- * one that ends inside a page) as its own positions [0, prefix_len[i]); its
- * own pages begin there.  A prefix stays as long as a stream shares it. */
+ * sees that prefix's first prefix_len[i] positions (any number that calls
+ * before have stored, also one that ends inside a page) as its own positions
+ * [0, prefix_len[i]); its own pages begin there.  A prefix stays, and is not
+ * released, as long as a stream shares it. */
 typedef struct cbx_kv_streams {
     int32_t  n_streams;        /* 1 .. 16384                                         */
     int32_t  n_prefix;         /* 0 .. n_streams                                     */
@@ -128,9 +129,15 @@ int cbx_kv_build(cbx_sampler* s, const cbx_kv_plan* p, void* stream);
  * are first stored at slot[r] (rows of one stream in one call see each other's);
  * without, the cache holds them already.  Rows without a position give zeros;
  * a row with a position whose page is not one of the pool's does not see those
- * positions; a row that sees none, or whose scores are all -inf, gives zeros.
- * Keys that a row does not see never reach it, whatever they hold.  Products,
- * sums and softmax statistics in fp32.
+ * positions; a row that sees none gives zeros.  Keys and values that a row does
+ * not see never reach it, whatever they hold.  A query or a seen key that is
+ * not finite leaves its own row's outputs undefined, no other's.
+ * Sums and softmax statistics are fp32.  Products are fp32's, or on the 16-bit
+ * matrix cores of values cut into parts: fp32 caches' into three bf16 parts
+ * (each product to 2^-21 of itself); fp16 caches' queries and weights into two
+ * fp16 parts (to 2^-22 and 2^-20 of themselves, or 2^-38 of the row's largest).
+ * n_rows * n_head, with tiles + n_tiles * cache->n_head, is at most 2^24 - 1,
+ * and n_pages * page_size * cache->n_head below 2^32 - 1 (CBX_ERR_UNSUPPORTED).
  * Step form with tiles: prefixes are read once for the rows of a tile; without:
  * by every row for itself, with the same result up to rounding. */
 typedef struct cbx_kv_attn {
@@ -144,7 +151,7 @@ typedef struct cbx_kv_attn {
     int64_t      ld_q;            /* >= 64 n_head, a multiple of 4                   */
     const float* k;               /* optional [n_rows][ld_kv], key head h at 64 h    */
     const float* v;               /* with k                                          */
-    int64_t      ld_kv;           /* >= 64 cache->n_head, a multiple of 4            */
+    int64_t      ld_kv;           /* >= 64 cache->n_head, a multiple of 4, < 2^31    */
     float*       out;             /* [n_rows][ld_out]                                */
     int64_t      ld_out;          /* >= 64 n_head, a multiple of 4                   */
     float        scale;

@@ -141,6 +141,25 @@ def test_tile_rows_and_workspace(lib):
     assert so.cbx_kv_workspace_bytes(ctypes.byref(a)) == 0  # prompts' rows are whole
 
 
+def test_grids_stay_within_a_launch(lib):
+    """Rows, tiles and the parts of both in one launch: 2^24 - 1 workgroups at most."""
+    mod, so, handle = lib
+    n, pages = 16384, (1 << 26) - 1  # 2^30 positions a stream, near enough: 64 parts a row are wanted
+    a = attn(mod, dict(t=dict(n_streams=n, n_prefix=1, max_pages=pages), r=dict(n_rows=n, n_tiles=n),
+                       a=dict(n_head=960, ld_q=960 * 64, ld_kv=320 * 64, ld_out=960 * 64),
+                       c=dict(n_head=320)))
+    a._keep[2].tile_rows = mod.Sampler.kv_tile_rows(960, 320)
+    assert n * 960 + n * 320 > 0xffffff
+    refused(mod, so.cbx_kv_attend(handle, ctypes.byref(a), None), mod.CBX_ERR_UNSUPPORTED)
+    assert so.cbx_kv_workspace_bytes(ctypes.byref(a)) == 0
+    a.n_head, a._keep[0].n_head, a._keep[2].n_tiles = 192, 64, 1024
+    a._keep[2].tile_rows = mod.Sampler.kv_tile_rows(192, 64)
+    parts = so.cbx_kv_workspace_bytes(ctypes.byref(a)) // (n * 192 * (64 * 4 + 8))
+    assert parts >= 2
+    shared = 1  # 1024 tiles of 64 key heads fill the card with a part each
+    assert 1024 * 64 * shared + (parts - shared) * n * 64 <= 0xffffff
+
+
 def z(*s, dt=torch.int32):
     return torch.zeros(s, dtype=dt)
 
