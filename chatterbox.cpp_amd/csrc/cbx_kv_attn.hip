@@ -1178,22 +1178,45 @@ constexpr int64_t kWaveUnits = 4096;
 
 int head_chunk(int group) { return group >= 3 ? 4 : group; }
 
+// Whether a key head's query heads are pairs of one tile.  us, vector units /
+// matrix cores, 16 fp16 heads, rows of 1000 keys: 2 heads a key head, 64 rows
+// 29.3 / 31.7; 4: 64 rows 25.9 / 21.6, 256 67.8 / 62.0; 8: 256 58.0 / 33.0.
+bool on_matrix(bool f16, int group) { return f16 && group >= 3; }
+
+// A row's workgroups (or waves) of one part.
+int row_units(bool f16, int n_kv, int group) {
+    const int G = head_chunk(group);
+    return n_kv * (on_matrix(f16, group) ? (group + 15) / 16 : (group + G - 1) / G);
+}
+
 Cut cut_of(const cbx_kv_attn& a) {
     Cut c{0, 0, kMinPart};
     if (a.rows->stream) return c;
     const int group = a.n_head / a.cache->n_head;
-    const int chunks = (group + head_chunk(group) - 1) / head_chunk(group);
-    const int64_t wgs = (int64_t)a.rows->n_rows * a.cache->n_head * chunks;
+    const bool f16 = a.cache->type == CBX_KV_F16;
+    const int64_t wgs = (int64_t)a.rows->n_rows * row_units(f16, a.cache->n_head, group);
     const int64_t cap = (int64_t)a.streams->max_pages * a.cache->page_size;
     const bool prefixes = a.streams->parent && a.streams->n_prefix > 0;
     const bool tiles = a.rows->tiles && prefixes;
     const int64_t longest = tiles || !prefixes ? cap : 2 * cap;
-    // parts worth a workgroup's start and end where there are enough of them
-    // (256 fp16 rows of 64 to 4001 keys, four query heads a key head: 143 us
-    // with 64 keys a part, 94 with 512)
-    c.min_part = (int)std::min<int64_t>(std::max<int64_t>(wgs / 2, kMinPart), 512);
-    int64_t own = (1024 + wgs - 1) / wgs;
-    own = std::max(own, (longest + 1023) / 1024);
+    // Parts worth a workgroup's start and end, and about as many workgroups as
+    // run at a time; of fp32 rows two such rounds where a part is still 256 keys,
+    // but none where whole rows fill a round (a join would come on top: 64 rows of
+    // 200 keys 19.4 / 24.2).  us: 256 fp16 rows of 64 to 4001 keys, four query heads a key
+    // head, parts of 64 keys and more 143, of 512 94; fp32 rows of 64 to 4001
+    // keys, one round / two: 8 rows 19.3 / 17.7, 16: 33.8 / 28.9, 32 with four
+    // heads a key head 34.6 / 28.8, 64: 57.7 / 38.9, but 16 of these (parts of 125)
+    // 21.6 / 23.8, and fp16 32 with four heads 20.4 / 22.8, 16 of 1000 keys with
+    // two 15.1 / 17.8
+    const bool two = !tiles && !f16 && wgs >= 128 && wgs < 1024;
+    c.min_part = two ? (int)std::min<int64_t>(std::max<int64_t>(wgs, 256), 512)
+                     : (int)std::min<int64_t>(std::max<int64_t>(wgs / 2, kMinPart), 512);
+    int64_t own = ((two ? 2048 : 1024) + wgs - 1) / wgs;
+    // a row of many keys in several parts whatever their number (us, parts of
+    // 2048 / 1024 / 512 / 256 keys: 256 fp32 rows of 64 to 4001 363 / 355 / 362 /
+    // 387); rounded, or rows of just over 1024 come in two halves (64 rows of
+    // 1000 97.4 / 92.5)
+    own = std::max(own, (longest + 512) / 1024);
     own = std::min(own, std::min<int64_t>(64, (longest + kMinPart - 1) / kMinPart));
     if (tiles) {
         const int64_t t = (int64_t)a.rows->n_tiles * a.cache->n_head;
@@ -1215,14 +1238,11 @@ Cut cut_of(const cbx_kv_attn& a) {
 // The step form: the rows' own keys, behind the prefixes' tiles where there are any.
 template <class T>
 hipError_t launch_step(const KvArgs& a, hipStream_t st) {
-    const int G = head_chunk(a.group), chunks = (a.group + G - 1) / G;
-    // a key head's query heads are pairs of one tile.  us, vector units / matrix
-    // cores, 16 fp16 heads, rows of 1000 keys: 2 heads a key head, 64 rows 29.3 /
-    // 31.7; 4: 64 rows 25.9 / 21.6, 256 67.8 / 62.0; 8: 256 58.0 / 33.0
-    const bool matrix = sizeof(T) == 2 && a.group >= 3;
+    const int G = head_chunk(a.group);
+    const bool matrix = on_matrix(sizeof(T) == 2, a.group);
     // beside prefixes' tiles a wave per row and head where those are many: four
     // heads a workgroup, no barrier
-    const int64_t units = (int64_t)a.n_rows * a.n_kv * (matrix ? (a.group + 15) / 16 : chunks);
+    const int64_t units = (int64_t)a.n_rows * row_units(sizeof(T) == 2, a.n_kv, a.group);
     const bool wave = !matrix && a.n_shared && units >= kWaveUnits;
     const unsigned blocks = (unsigned)(wave ? (units + 3) / 4 : units), cuts = (unsigned)max(a.n_own, 1);
     const unsigned tiles = (unsigned)a.n_kv * a.n_tiles * a.n_shared;
