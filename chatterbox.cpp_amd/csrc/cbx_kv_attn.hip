@@ -573,8 +573,8 @@ struct Walk {
 // time fp32, 60 % fp16) and the matrix cores' (43 %, 29 %) together.  64 prompts
 // of 129 to 383 rows fp32 129 us, 3.1 TB/s; 8 of 301 to 1501 fp16 behind 377 keys
 // 124.  Fewer instructions for a stage's addresses, all of K's reads before the
-// products, 8 waves a workgroup and two sets of pairs a wave were no faster or
-// slower; what was: stages loaded behind the choice of their addresses (fp16
+// products, 8 waves a workgroup, two sets of pairs a wave and 32 pairs a wave on
+// 32x32 products (804 us for the 530) were no faster or slower; what was faster: stages loaded behind the choice of their addresses (fp16
 // 8 %), the longest tiles first (7 %), four workgroups a CU for fp16 (8 %).
 enum { kPrompt, kPrefix, kOneRow };
 template <class T, bool SPLIT, int FORM>

@@ -321,6 +321,15 @@ def test_shared_prefix_matches_oracle(cbx, prefixes, children, dtype, n_kv, grou
     run(cbx, d, r2, plan, c, n_kv, group, rng, q=x["q"], kn=x["kn"], vn=x["vn"])
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("group", [1, 2, 5])
+def test_many_rows_beside_prefixes(cbx, dtype, group):
+    """More rows than workgroups are given one each (a wave a row and key head,
+    but for fp16 with three and more query heads), some without a prefix."""
+    children = [((-1, 0), (0, 140), (1, 17))[i % 3] + (i % 37,) for i in range(1040)]
+    test_shared_prefix_matches_oracle(cbx, [150, 17], children, dtype, 4, group, 16)
+
+
 PROMPTS = [  # prefixes, (prefix, shared, already cached, new)
     ([], [(-1, 0, 0, 1)]), ([], [(-1, 0, 0, 16)]), ([], [(-1, 0, 0, 17), (-1, 0, 0, 63)]),
     ([], [(-1, 0, 5, 64), (-1, 0, 16, 65), (-1, 0, 40, 3), (-1, 0, 0, 0), (-1, 0, 9, 129)]),
@@ -360,6 +369,13 @@ def test_prompts_match_oracle(cbx, prefixes, streams, dtype, n_kv, group, page):
     r = d.rows(False, sum(new) + 5, tile_rows=mod.Sampler.kv_tile_rows(n_kv * group, n_kv))
     plan = d.plan(s, r, n_new=new)
     run(cbx, d, r, plan, c, n_kv, group, rng, sd=2.0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_prompts_behind_long_caches(cbx, dtype):
+    """Whole tiles a workgroup over many stages: cached keys, then new ones."""
+    test_prompts_match_oracle(cbx, [77], [(0, 70, 523, 130), (-1, 0, 700, 129)] * 12, dtype,
+                              8, 1, 16)
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16"])

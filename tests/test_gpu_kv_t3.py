@@ -201,3 +201,41 @@ def test_refusals(small):
         s.t3_kv(dm, srv.cache, srv.streams, r, hid[:3], tokens=tok)
     with pytest.raises(ValueError):
         s.t3_kv(dm, srv.cache, srv.streams, r, hid, tokens=tok.long())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_a_step_captured_with_its_plan(small, dtype):
+    """Plan and transformer in one graph, replayed past a page's end while its
+    streams grow, eager calls of another server on the handle between: each
+    replay's rows are the eager steps' of a server like it."""
+    torch, mod, s, dm, rm = small
+    made = []
+    for _ in range(3):
+        rng = np.random.default_rng(8)
+        torch.manual_seed(9)
+        srv = Server(torch, mod, s, dm, 9, 1, getattr(torch, dtype))
+        srv.prompt((rng.standard_normal((21, N)) * 0.7).astype(np.float32), [21] + [0] * 8)
+        srv.prefix_len.copy_(srv.ints([0] + [21] * 4 + [10] * 4))
+        srv.parent.copy_(srv.ints([-1] + [0] * 8))
+        srv.prompt((rng.standard_normal((72, N)) * 0.7).astype(np.float32), [0] + [9] * 8)
+        made.append(srv)
+    eager, captured, other = made
+    state = [1] + [0] * 8
+    r = captured.rows(9, step=True)
+    tokens, hid = captured.ints([0] * 9), torch.zeros((9, N), device="cuda")
+    plan = mod.Sampler.kv_plan(captured.streams, r, page_size=16, state=captured.ints(state))
+    print(f"[gpu-case] captured step {dtype}", flush=True)
+    other.step([1] * 9, state, True)  # the handle's workspace, as large as the graph's call wants it
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.kv_build(plan)
+        s.t3_kv(dm, captured.cache, captured.streams, r, hid, tokens=tokens)
+    for _ in range(12):
+        ids = rng.integers(0, V, 9)
+        want = eager.step(ids, state, True)
+        other.step(rng.integers(0, V, 9), state, True)
+        tokens.copy_(captured.ints(ids))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(hid.cpu().numpy(), want)
+    assert torch.equal(captured.length, eager.length) and captured.length.tolist()[1:] == [21] * 8
