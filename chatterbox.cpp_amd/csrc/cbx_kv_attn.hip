@@ -632,12 +632,18 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         dead_rows();
         return;
     }
-    const int p = p0 + (SPLIT ? 0 : 16 * w) + c;
-    const int local = over_group(a, p), at = first + local, h = kvh * a.group + p - local * a.group;
-    bool real = p < pairs && at < a.n_rows;
-    int row = -1;
-    if (real) row = FORM == kPrefix ? a.order[at] : at;
-    real = real && row >= 0 && row < a.n_rows;
+    // the row of a lane's pair (-1: none), its query head
+    const auto pair_of = [&](int lane_of, int& h, int wave) {
+        const int p = p0 + (SPLIT ? 0 : 16 * wave) + (lane_of & 15);
+        const int local = over_group(a, p), at = first + local;
+        h = kvh * a.group + p - local * a.group;
+        int row = -1;
+        if (p < pairs && at < a.n_rows) row = FORM == kPrefix ? a.order[at] : at;
+        return row < a.n_rows ? row : -1;
+    };
+    int h;
+    const int row = pair_of(lane, h, w);
+    const bool real = row >= 0;
     const int rc = real ? row : 0;
     // the walk, and lim, the last key the pair sees
     const int cap = a.max_pages << a.shift;
@@ -904,11 +910,14 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     float ref = -INFINITY, off = kUp, bar = -INFINITY;
     f4 sum = f4{0.0f, 0.0f, 0.0f, 0.0f};  // the first of it
     int last = lim, least = real ? lim : INT32_MAX;
-#pragma unroll
-    for (int x = 1; x < 16; x <<= 1) {
-        last = max(last, __shfl_xor(last, x));
-        least = min(least, __shfl_xor(least, x));
-    }
+    const auto over = [&](auto x) {  // lanes at a distance of x
+        last = max(last, __builtin_amdgcn_ds_swizzle(last, x << 10 | 0x1f));
+        least = min(least, __builtin_amdgcn_ds_swizzle(least, x << 10 | 0x1f));
+    };
+    over(std::integral_constant<int, 1>());
+    over(std::integral_constant<int, 2>());
+    over(std::integral_constant<int, 4>());
+    over(std::integral_constant<int, 8>());
     last = __builtin_amdgcn_readfirstlane(last);
     least = __builtin_amdgcn_readfirstlane(least);
 
@@ -1079,40 +1088,46 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         if (more) store(kBufs == 2 ? (t + 1) & 1 : 0, (t + 1) % 3);
         __syncthreads();
     }
+    // what the lane stands for once more: kept over the loop it would cost registers
+    int tid_end = tid;
+    asm volatile("" : "+v"(tid_end));
+    const int ge = tid_end >> 4 & 3, ce = tid_end & 15, we = tid_end >> 6;
+    int h_end;
+    const int row_end = pair_of(tid_end & 63, h_end, we);
     // through LDS into rows: [16 w + pair][dimension]
-    float* const os = reinterpret_cast<float*>(lds) + 16 * w * kPad;
+    float* const os = reinterpret_cast<float*>(lds) + 16 * we * kPad;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        *reinterpret_cast<f4*>(os + c * kPad + 16 * i + 4 * g) = o[i];
+        *reinterpret_cast<f4*>(os + ce * kPad + 16 * i + 4 * ge) = o[i];
     }
-    if (g == 0) {
-        join_m[w][c] = ref;
-        join_s[w][c] = sum[0];
+    if (ge == 0) {
+        join_m[we][ce] = ref;
+        join_s[we][ce] = sum[0];
     }
     __syncthreads();
     // lane (g, c): dimensions 4 c .. of pair i
     const auto finish = [&](int i, float pm, float ps, const f4& po) {
-        const int ri = __shfl(real ? row : a.n_rows, i), hi = __shfl(h, i);
+        const int ri = __shfl(row_end >= 0 ? row_end : a.n_rows, i), hi = __shfl(h_end, i);
         if (FORM == kPrefix || (FORM == kOneRow && a.n_own > 0)) {
             if (ri >= a.n_rows) return;
             constexpr float kDown = F16 ? 1.0f / 16384.0f : 1.0f;
             const int part = (FORM == kPrefix ? a.n_own : 0) + cut;
             const int64_t to = ((int64_t)part * a.n_rows + ri) * a.n_head + hi;
-            if (c == 0) a.part_ms[to] = float2{pm, __fmul_rn(ps, kDown)};
-            *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * c) = po * kDown;
+            if (ce == 0) a.part_ms[to] = float2{pm, __fmul_rn(ps, kDown)};
+            *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * ce) = po * kDown;
         } else {
             const float over = ps == 0.0f ? 0.0f : __fdiv_rn(1.0f, ps);
-            attn_store4(a.o, a.n_rows, ri, hi, c, po * over);
+            attn_store4(a.o, a.n_rows, ri, hi, ce, po * over);
         }
     };
     if constexpr (!SPLIT) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const int i = 4 * t + g;
-            finish(i, join_m[w][i], join_s[w][i], *reinterpret_cast<const f4*>(os + i * kPad + 4 * c));
+            const int i = 4 * t + ge;
+            finish(i, join_m[we][i], join_s[we][i], *reinterpret_cast<const f4*>(os + i * kPad + 4 * ce));
         }
     } else {  // wave w joins the four waves' pairs 4 w + g
-        const int i = 4 * w + g;
+        const int i = 4 * we + ge;
         float M = join_m[0][i];
 #pragma unroll
         for (int x = 1; x < 4; ++x) M = fmaxf(M, join_m[x][i]);
@@ -1122,7 +1137,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         for (int x = 0; x < 4; ++x) {
             const float f = rescale(join_m[x][i], M);
             st = __fadd_rn(st, __fmul_rn(join_s[x][i], f));
-            const f4 ov = *reinterpret_cast<const f4*>(reinterpret_cast<float*>(lds) + (16 * x + i) * kPad + 4 * c);
+            const f4 ov = *reinterpret_cast<const f4*>(reinterpret_cast<float*>(lds) + (16 * x + i) * kPad + 4 * ce);
 #pragma unroll
             for (int e = 0; e < 4; ++e) ot[e] = __fadd_rn(ot[e], __fmul_rn(ov[e], f));
         }
