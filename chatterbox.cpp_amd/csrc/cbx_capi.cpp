@@ -37,6 +37,14 @@ struct cbx_sampler {
     // the T3 decode step's workspace, grown on demand
     void* d_t3 = nullptr;
     size_t t3_bytes = 0;
+    // whether a call that uses these was captured, and the buffers replaced
+    // since, which its graph still holds
+    struct Kept {
+        void* p;
+        Kept* next;
+    };
+    bool captured = false;
+    Kept* kept = nullptr;
     // Pinned host memory that the single-row kernels read and write in place
     // (coherent: nothing of an earlier call stays in a cache): the row, the
     // unconditional row, the history, the allowed words, then the rest.  Over
@@ -120,9 +128,42 @@ void release(cbx_sampler* s) {
     (void)hipFree(s->d_redo_row);
     (void)hipFree(s->d_head);
     (void)hipFree(s->d_t3);
+    while (s->kept) {
+        cbx_sampler::Kept* const k = s->kept;
+        s->kept = k->next;
+        (void)hipFree(k->p);
+        delete k;
+    }
     if (s->h_row) (void)hipHostFree(s->h_row);
     if (s->stream) (void)hipStreamDestroy(s->stream);
     delete s;
+}
+
+// One of the handle's buffers for a call of `need` bytes on st: replaced by a
+// larger one where it is too small, but not while st is captured.
+int grow(const char* fn, cbx_sampler* s, void** p, size_t* bytes, size_t need, hipStream_t st) {
+    hipStreamCaptureStatus c = hipStreamCaptureStatusNone;
+    if (st && hipStreamIsCapturing(st, &c) != hipSuccess) (void)hipGetLastError();
+    const bool capturing = c == hipStreamCaptureStatusActive;
+    if (need > *bytes) {
+        if (capturing)
+            return fail(CBX_ERR_UNSUPPORTED, "%s: the handle's buffer has %zu of %zu bytes: make a "
+                        "call of this size before one is captured", fn, *bytes, need);
+        if (s->captured && *p) {
+            cbx_sampler::Kept* const k = new (std::nothrow) cbx_sampler::Kept{*p, s->kept};
+            if (!k) return fail(CBX_ERR_NOMEM, "%s: out of host memory", fn);
+            s->kept = k;
+        } else {
+            CBX_HIP(hipDeviceSynchronize());
+            CBX_HIP(hipFree(*p));
+        }
+        *p = nullptr;
+        *bytes = 0;
+        CBX_HIP(hipMalloc(p, need));
+        *bytes = need;
+    }
+    s->captured = s->captured || (capturing && need);
+    return CBX_OK;
 }
 
 // Survivor capacity for a launch: the smaller of n_vocab and the caller's
@@ -495,14 +536,8 @@ int check_head(const char* fn, const cbx_head* h, int32_t n_rows, int32_t n_voca
 int run_head(cbx_sampler* s, const cbx_head* h, int32_t n_rows, int32_t n_vocab,
              int64_t ld_logits, hipStream_t st) {
     const size_t need = cbx::head_scratch_bytes(n_rows, h->hidden_uncond != nullptr, h->n_embd);
-    if (need > s->head_bytes) {
-        CBX_HIP(hipDeviceSynchronize());
-        CBX_HIP(hipFree(s->d_head));
-        s->d_head = nullptr;
-        s->head_bytes = 0;
-        CBX_HIP(hipMalloc(&s->d_head, need));
-        s->head_bytes = need;
-    }
+    const int rc = grow("speech_head", s, &s->d_head, &s->head_bytes, need, st);
+    if (rc != CBX_OK) return rc;
     CBX_HIP(cbx::launch_head(h->weights, h->wtype, h->bias, h->hidden, h->hidden_uncond,
                              h->ld_hidden, h->logits, h->logits_uncond, ld_logits, n_rows,
                              n_vocab, h->n_embd, s->d_head, st));
@@ -742,14 +777,8 @@ int t3_run(const char* fn, cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows
     }
     DeviceGuard g(s->device);
     const size_t body = cbx::t3_workspace_bytes(n_rows, m->n_embd), need = body + kv_bytes;
-    if (need > s->t3_bytes) {
-        CBX_HIP(hipDeviceSynchronize());
-        CBX_HIP(hipFree(s->d_t3));
-        s->d_t3 = nullptr;
-        s->t3_bytes = 0;
-        CBX_HIP(hipMalloc(&s->d_t3, need));
-        s->t3_bytes = need;
-    }
+    const int rc = grow(fn, s, &s->d_t3, &s->t3_bytes, need, (hipStream_t)stream);
+    if (rc != CBX_OK) return rc;
     if (kv) a.workspace = static_cast<char*>(s->d_t3) + body;
     CBX_HIP(cbx::launch_t3_step(*m, n_rows, tokens, inputs, positions, state, slots, n_slots,
                                 *cache, hidden, s->d_t3, (hipStream_t)stream, kv ? &a : nullptr));

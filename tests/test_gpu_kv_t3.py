@@ -230,7 +230,11 @@ def test_a_step_captured_with_its_plan(small, dtype):
     with torch.cuda.graph(graph):
         s.kv_build(plan)
         s.t3_kv(dm, captured.cache, captured.streams, r, hid, tokens=tokens)
-    for _ in range(12):
+    for i in range(12):
+        if i == 5:  # a call that wants a larger workspace than the graph's
+            k = 133 if dtype == "float32" else 145
+            big = Server(torch, mod, s, dm, 9, 0, torch.float32, n_pages=100)
+            big.prompt((rng.standard_normal((9 * k, N)) * 0.7).astype(np.float32), [k] * 9)
         ids = rng.integers(0, V, 9)
         want = eager.step(ids, state, True)
         other.step(rng.integers(0, V, 9), state, True)
@@ -239,3 +243,24 @@ def test_a_step_captured_with_its_plan(small, dtype):
         torch.cuda.synchronize()
         assert np.array_equal(hid.cpu().numpy(), want)
     assert torch.equal(captured.length, eager.length) and captured.length.tolist()[1:] == [21] * 8
+
+
+def test_a_workspace_does_not_grow_in_a_capture(small):
+    torch, mod, s, dm, rm = small
+    fresh = mod.Sampler(device=0, max_vocab=1024, max_history=64)
+    srv = Server(torch, mod, s, dm, 9, 0, torch.float32)
+    r = srv.rows(9, step=True)
+    srv.plan(r)
+    hid, x = torch.full((9, N), 7.0, device="cuda"), torch.zeros(8, device="cuda")
+    tokens = srv.ints([1] * 9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1.0)
+        with pytest.raises(mod.CbxError):
+            fresh.t3_kv(dm, srv.cache, srv.streams, r, hid, tokens=tokens)
+    graph.replay()
+    fresh.t3_kv(dm, srv.cache, srv.streams, r, hid, tokens=tokens)
+    torch.cuda.synchronize()
+    assert torch.all(x == 1.0) and torch.isfinite(hid).all() and not torch.any(hid == 7.0)
+    fresh.close()
