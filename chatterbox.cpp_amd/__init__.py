@@ -470,6 +470,7 @@ class Sampler:
         h = ctypes.c_void_p()
         _check(self.lib.cbx_sampler_create(ctypes.byref(h), device, max_vocab, max_history))
         self.handle = h
+        self.device = device
 
     def close(self):
         if getattr(self, "handle", None):
@@ -678,6 +679,7 @@ class Sampler:
         [n_rows, n_embd] out."""
         import torch
         n, f = rows.n_rows, torch.float32
+        self._on_device("t3_kv", streams)
         dev = self._one_call("t3_kv", streams, rows)
         if cache._tensors[0].device != dev:
             raise ValueError("t3_kv: the cache is on another device")
@@ -775,6 +777,12 @@ class Sampler:
         """cbx_kv_tile_rows: rows of a tile."""
         return load_library().cbx_kv_tile_rows(n_head, n_kv_head)
 
+    def _on_device(self, fn, streams):
+        dev = streams._tensors[0].device
+        if dev.type != "cuda" or dev.index != self.device:
+            raise ValueError("%s: the tables are on %s, the handle is of GPU %d" % (
+                fn, dev, self.device))
+
     @staticmethod
     def _one_call(fn, streams, rows):
         n = streams.n_streams
@@ -806,6 +814,7 @@ class Sampler:
 
     def kv_build(self, plan, stream=None):
         """cbx_kv_build: the plan's page tables, rows and tiles."""
+        self._on_device("kv_build", plan._tensors[0])
         st = _stream_ptr() if stream is None else ctypes.c_void_p(stream)
         _check(self.lib.cbx_kv_build(self.handle, ctypes.byref(plan), st))
 
@@ -854,6 +863,7 @@ class Sampler:
     def kv_attend(self, attn, stream=None):
         """cbx_kv_attend: attention of one layer's rows, their new keys and
         values stored first."""
+        self._on_device("kv_attend", attn._tensors[1])
         st = _stream_ptr() if stream is None else ctypes.c_void_p(stream)
         _check(self.lib.cbx_kv_attend(self.handle, ctypes.byref(attn), st))
 

@@ -152,7 +152,7 @@ typedef struct cbx_kv_attn {
     const float* k;               /* optional [n_rows][ld_kv], key head h at 64 h    */
     const float* v;               /* with k                                          */
     int64_t      ld_kv;           /* >= 64 cache->n_head, a multiple of 4, < 2^31    */
-    float*       out;             /* [n_rows][ld_out]                                */
+    float*       out;             /* [n_rows][ld_out], apart from q, k and v         */
     int64_t      ld_out;          /* >= 64 n_head, a multiple of 4                   */
     float        scale;
     void*        workspace;       /* cbx_kv_workspace_bytes of this call; 16-byte

@@ -207,3 +207,18 @@ def test_python_view_refuses(lib):
         with pytest.raises(ValueError):
             S.kv_attn(c, t, r, bad.pop("q"), bad.pop("out"), **bad)
     S.kv_attn(c, t, r, q, o, k=z(4, 192, dt=f), v=z(4, 192, dt=f))
+
+
+def test_host_tensors_are_refused(lib):
+    """Structures over host memory are made (their shapes are checked) and not run."""
+    mod, so, _ = lib
+    S, c, t, r = view(mod)
+    s = object.__new__(S)
+    s.lib, s.handle, s.device = so, None, 0
+    with pytest.raises(ValueError, match="GPU 0"):
+        s.kv_build(S.kv_plan(t, r, page_size=16))
+    q = z(4, 192, dt=torch.float32)
+    with pytest.raises(ValueError, match="GPU 0"):
+        s.kv_attend(S.kv_attn(c, t, r, q, torch.empty_like(q)))
+    with pytest.raises(ValueError, match="GPU 0"):
+        s.t3_kv(mod.T3Model(), c, t, r, q, tokens=z(4))
