@@ -572,10 +572,12 @@ struct Walk {
 // of the parts'), fp16 530 (260, 585): the vector units' instructions (half the
 // time fp32, 60 % fp16) and the matrix cores' (43 %, 29 %) together.  64 prompts
 // of 129 to 383 rows fp32 129 us, 3.1 TB/s; 8 of 301 to 1501 fp16 behind 377 keys
-// 124.  Fewer instructions for a stage's addresses, all of K's reads before the
-// products, 8 waves a workgroup, two sets of pairs a wave and 32 pairs a wave on
-// 32x32 products (804 us for the 530) were no faster or slower; what was faster: stages loaded behind the choice of their addresses (fp16
-// 8 %), the longest tiles first (7 %), four workgroups a CU for fp16 (8 %).
+// 124.  What made them faster: loads that stand behind the choice of their
+// addresses (fp16 8 %), the longest tiles first (7 %), four workgroups a CU for
+// fp16 (8 %), nothing kept over the loop that its end can find again (up to
+// 7 %).  What did not: fewer instructions for a stage's addresses, all of K's
+// reads before the products, 8 waves a workgroup, two sets of pairs a wave, 32
+// pairs a wave on 32x32 products (804 us where these take 530).
 enum { kPrompt, kPrefix, kOneRow };
 template <class T, bool SPLIT, int FORM>
 __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32_t blocks, int cut) {
@@ -1151,6 +1153,8 @@ __global__ __launch_bounds__(256) void kv_rows(KvArgs a) {
     rows_of<T, G, 4>(a, blockIdx.x, blockIdx.y);
 }
 
+// Workgroups a CU: fp16 stages leave room for four (three: 131 us where four take
+// 120, 8 prompts behind a voice), fp32 ones' LDS for three.
 template <class T, bool SPLIT, int FORM>
 __global__ __launch_bounds__(256, SPLIT ? 2 : sizeof(T) == 2 ? 4 : 3) void kv_tiles(KvArgs a) {
     tiles_of<T, SPLIT, FORM>(a, blockIdx.x, gridDim.x, blockIdx.y);
