@@ -681,6 +681,7 @@ class Sampler:
         n, f = rows.n_rows, torch.float32
         self._on_device("t3_kv", streams)
         dev = self._one_call("t3_kv", streams, rows)
+        rows = self._with_tiles(streams, rows)
         if cache._tensors[0].device != dev:
             raise ValueError("t3_kv: the cache is on another device")
         self._check_kv("t3_kv", dev, hidden=(hidden, f, (n, model.n_embd)),
@@ -754,7 +755,8 @@ class Sampler:
         """A cbx_kv_rows over device int32 tensors: position, slot (and stream:
         the prompt form) [n_rows], row_start and page_start [n_streams + 1],
         counts [4], optional tiles [n_tiles, 4] and, in the step form with
-        tiles, order [n_rows]."""
+        tiles, order [n_rows].  Prompts attend with no tiles too, or with too
+        few for cbx_kv_build to fill: the attention then finds its own."""
         import torch
         n, i = position.numel(), torch.int32
         Sampler._check_kv("kv_rows", position=(position, i, (n,)), slot=(slot, i, (n,)),
@@ -776,6 +778,17 @@ class Sampler:
     def kv_tile_rows(n_head, n_kv_head):
         """cbx_kv_tile_rows: rows of a tile."""
         return load_library().cbx_kv_tile_rows(n_head, n_kv_head)
+
+    @staticmethod
+    def _with_tiles(streams, rows):
+        """rows, or, where a prompt's tiles are fewer than its rows can need, a
+        copy without them."""
+        if not rows.stream or rows.tile_rows < 1 or \
+                rows.n_tiles >= rows.n_rows // rows.tile_rows + streams.n_streams:
+            return rows
+        r = KvRows.from_buffer_copy(rows)
+        r.tiles, r.n_tiles, r._tensors = None, 0, rows._tensors
+        return r
 
     def _on_device(self, fn, streams):
         dev = streams._tensors[0].device
@@ -827,6 +840,7 @@ class Sampler:
         given (uint8): two calls that may run at once take a KvAttn each."""
         import torch
         dev = Sampler._one_call("kv_attn", streams, rows)
+        rows = Sampler._with_tiles(streams, rows)
         if cache._tensors[0].device != dev:
             raise ValueError("kv_attn: the cache is on another device")
         n = rows.n_rows

@@ -660,14 +660,16 @@ int check_kv_attn(const char* fn, const cbx_kv_attn* a) {
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||
         !aligned16(c.k) || !aligned16(c.v) || !aligned16(a->workspace))
         return fail(CBX_ERR_INVALID, "%s: an address is not 16-byte aligned", fn);
-    if (a->rows->stream && !a->rows->tiles)
-        return fail(CBX_ERR_INVALID, "%s: the prompt form's tiles are NULL", fn);
-    if (a->rows->tiles && a->rows->tile_rows != cbx_kv_tile_rows(a->n_head, c.n_head))
-        return fail(CBX_ERR_INVALID, "%s: tile_rows %d, %d wanted", fn, a->rows->tile_rows,
-                    cbx_kv_tile_rows(a->n_head, c.n_head));
+    if (a->rows->stream && !a->rows->tiles && a->rows->n_tiles != 0)
+        return fail(CBX_ERR_INVALID, "%s: %d tiles of the prompt form are NULL", fn, a->rows->n_tiles);
+    const int32_t tile_rows = cbx_kv_tile_rows(a->n_head, c.n_head);
+    if (a->rows->tiles && a->rows->tile_rows != tile_rows)
+        return fail(CBX_ERR_INVALID, "%s: tile_rows %d, %d wanted", fn, a->rows->tile_rows, tile_rows);
+    const int64_t n_tiles = a->rows->tiles    ? a->rows->n_tiles
+                            : a->rows->stream ? (int64_t)a->rows->n_rows / tile_rows + a->streams->n_streams
+                                              : 0;
     // the launches' grids: 2^24 workgroups of 256 at most
-    if ((int64_t)a->rows->n_rows * a->n_head +
-            (a->rows->tiles ? (int64_t)a->rows->n_tiles * c.n_head : 0) > cbx::kMaxKvGrid)
+    if ((int64_t)a->rows->n_rows * a->n_head + n_tiles * c.n_head > cbx::kMaxKvGrid)
         return fail(CBX_ERR_UNSUPPORTED, "%s: %d rows of %d heads", fn, a->rows->n_rows, a->n_head);
     return CBX_OK;
 }

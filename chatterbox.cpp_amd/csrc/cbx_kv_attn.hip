@@ -579,6 +579,26 @@ struct Walk {
 // reads before the products, 8 waves a workgroup, two sets of pairs a wave, 32
 // pairs a wave on 32x32 products (804 us where these take 530).
 enum { kPrompt, kPrefix, kOneRow };
+
+// Tile t of prompts that come without a list of them, as the plan would have
+// written it (count 0 or less: none): stream i's tiles have the numbers from
+// row_start[i] / tile_rows + i on, so none of them reaches the next stream's first
+// and t is below n_rows / tile_rows + n_streams.  Every lane of the wave takes
+// part: 64 streams are tried at a time.
+__device__ __forceinline__ int4 tile_of(const KvArgs& a, int t) {
+    const int lane = threadIdx.x & 63, T = a.tile_rows;
+    int i = 0, end = a.n_streams;
+    while (end - i > 1) {  // the last stream of [i, end) whose first number is at most t
+        const int step = (end - i + 63) / 64, x = i + lane * step;
+        const bool on = x < end && a.row_start[min(x, end - 1)] / T + x <= t;
+        i += max((int)__popcll(__ballot(on)) - 1, 0) * step;
+        end = min(i + step, end);
+    }
+    const int r0 = a.row_start[i], r1 = min(a.row_start[i + 1], a.n_rows);
+    const int first = min(max(r0 + (t - r0 / T - i) * T, 0), a.n_rows), count = min(T, r1 - first);
+    return make_int4(i, first, count, count > 0 ? a.position[first + count - 1] + 1 : 0);
+}
+
 template <class T, bool SPLIT, int FORM>
 __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32_t blocks, int cut) {
     constexpr bool F16 = sizeof(T) == 2, PROMPT = FORM == kPrompt;
@@ -622,7 +642,8 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         count = 1;
         keys = 0;
     } else {
-        const int4 tile = a.tiles[PROMPT ? a.n_tiles - 1 - (SPLIT ? unit / 4 : unit) : unit];
+        const int t = PROMPT ? a.n_tiles - 1 - (SPLIT ? unit / 4 : unit) : unit;
+        const int4 tile = PROMPT && !a.tiles ? tile_of(a, t) : a.tiles[t];
         who = __builtin_amdgcn_readfirstlane(tile.x);
         first = min(max(__builtin_amdgcn_readfirstlane(tile.y), 0), a.n_rows);
         count = min(__builtin_amdgcn_readfirstlane(tile.z), a.tile_rows);
@@ -1332,8 +1353,9 @@ hipError_t launch_kv_attend(const cbx_kv_attn& c, uint32_t* parts, float* inv, h
     a.parent = s.parent;
     a.prefix_len = s.prefix_len;
     a.n_rows = r.n_rows;
-    a.n_tiles = r.n_tiles;
-    a.tile_rows = r.tile_rows;
+    const bool listed = !r.stream || r.tiles;  // prompts' tiles, else found by their numbers
+    a.tile_rows = listed ? r.tile_rows : cbx_kv_tile_rows(c.n_head, p.n_head);
+    a.n_tiles = listed ? r.n_tiles : r.n_rows / a.tile_rows + s.n_streams;
     a.row_start = r.row_start;
     a.position = r.position;
     a.slot = r.slot;

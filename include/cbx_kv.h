@@ -82,11 +82,12 @@ typedef struct cbx_kv_rows {
     int32_t* row_start;  /* [n_streams + 1] new rows before each stream              */
     int32_t* page_start; /* [n_streams + 1] pages taken before each stream           */
     int32_t* counts;     /* [4] rows, tiles, pages taken, streams refused            */
-    int32_t* tiles;      /* [n_tiles][4] stream, first row, rows, keys.  Prompt form
-                            (required to attend): tile_rows rows of one stream, keys
-                            [0, keys).  Step form (optional): rows that share the
-                            prefix `stream`, entries [first, first + rows) of order,
-                            keys the longest of their prefixes.  Unused: -1, 0, 0, 0 */
+    int32_t* tiles;      /* [n_tiles][4] stream, first row, rows, keys.  Prompt form:
+                            tile_rows rows of one stream, keys [0, keys); NULL with
+                            n_tiles 0: the attention finds them from row_start.
+                            Step form (optional): rows that share the prefix
+                            `stream`, entries [first, first + rows) of order, keys
+                            the longest of their prefixes.  Unused: -1, 0, 0, 0      */
     int32_t* order;      /* step form with tiles: [n_rows] the rows that share a
                             prefix, by prefix, then -1                               */
 } cbx_kv_rows;
@@ -136,7 +137,8 @@ int cbx_kv_build(cbx_sampler* s, const cbx_kv_plan* p, void* stream);
  * matrix cores of values cut into parts: fp32 caches' into three bf16 parts
  * (each product to 2^-21 of itself); fp16 caches' queries and weights into two
  * fp16 parts (to 2^-22 and 2^-20 of themselves, or 2^-38 of the row's largest).
- * n_rows * n_head, with tiles + n_tiles * cache->n_head, is at most 2^24 - 1,
+ * n_rows * n_head, with tiles + n_tiles * cache->n_head (prompts without a list:
+ * as many as it would have), is at most 2^24 - 1,
  * and n_pages * page_size * cache->n_head below 2^32 - 1 (CBX_ERR_UNSUPPORTED).
  * Step form with tiles: prefixes are read once for the rows of a tile; without:
  * by every row for itself, with the same result up to rounding. */

@@ -1,0 +1,85 @@
+"""GPU tests of the paged cache's calls that its documentation allows beside the
+usual ones, against the same oracle, within the same bound (test_gpu_kv.py)."""
+import numpy as np
+import pytest
+
+from oracle import cbx_kv_oracle as KV
+from test_gpu_kv import D, Dev, caches, cbx, run, say, store  # noqa: F401
+from test_gpu_kv_t3 import N, Server, small  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def pool_of(rng, lens, page, n_prefix=0, parent=None, prefix_len=None, extra=2):
+    """Room for lens positions and one more of each stream."""
+    n_pages = sum(-(-(x + 1) // page) for x in lens) + extra
+    return KV.Pool(len(lens), max(-(-(max(lens) + 1) // page), 1), page, n_pages, n_prefix=n_prefix,
+                   parent=parent, prefix_len=prefix_len, free=rng.permutation(n_pages))
+
+
+# ------------------------------------------------------------------ prompts without a list of tiles
+
+UNLISTED = [  # (already cached, new) of each stream, key heads, heads a key head, prefix or 0
+    ([(0, 1)], 2, 1, 0), ([(0, 251)], 4, 1, 0),
+    ([(5, 64), (16, 65), (40, 3), (0, 0), (9, 129)], 2, 1, 45),
+    ([(0, 0), (0, 0), (3, 7), (0, 0)], 1, 5, 20),
+    ([(3, i % 3) for i in range(70)], 1, 3, 0),
+    ([(0, 9)] * 3 + [(0, 0)] * 61 + [(1, 30)], 1, 64, 0),
+    ([(0, (1, 0, 0, 2)[i % 4]) for i in range(4200)], 1, 1, 0),  # three rounds of 64 streams
+    ([(100, 130)] * 24, 8, 1, 0),  # whole tiles a workgroup
+]
+
+
+@pytest.mark.parametrize("short", [False, True], ids=["none", "too-few"])
+@pytest.mark.parametrize("streams,n_kv,group,prefix", UNLISTED,
+                         ids=[f"{len(x[0])}x{x[0][0][1]}-{x[2]}" for x in UNLISTED])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_prompts_without_a_list_of_tiles(cbx, streams, n_kv, group, prefix, dtype, short):  # noqa: F811
+    """Rows planned without tiles, or given to the attention with fewer than they
+    need: the outputs are those with the plan's list, bit for bit, and the oracle's."""
+    torch, mod, s = cbx
+    rng = np.random.default_rng(len(streams) + group)
+    n0 = 1 if prefix else 0
+    had = [prefix] * n0 + [x[0] for x in streams]
+    new = [0] * n0 + [x[1] for x in streams]
+    n = len(had)
+    say("no list", len(streams), streams[0], n_kv, group, dtype, short)
+    pool = pool_of(rng, [a + b for a, b in zip(had, new)], 16, n0, [-1] * n0 + [n0 - 1] * len(streams),
+                   [0] * n0 + [prefix] * len(streams))
+    d = Dev(torch, mod, pool)
+    if sum(had):
+        d.plan(s, d.rows(False, sum(had)), n_new=had)
+    c = caches(torch, rng, pool, n_kv, getattr(torch, dtype))
+    store(torch, rng, pool, c, 0, had)
+    T = mod.Sampler.kv_tile_rows(n_kv * group, n_kv)
+    listed = d.rows(False, sum(new) + 5, tile_rows=T)
+    plan = d.plan(s, listed, n_new=new)
+    want, x = run(cbx, d, listed, plan, c, n_kv, group, rng, sd=2.0)
+    b = {k: t for k, t in listed.b.items() if k != "tiles"}
+    if short:
+        b["tiles"] = listed.b["tiles"][:-1].fill_(-1)
+    r = mod.Sampler.kv_rows(**b, tile_rows=T if short else 0)
+    got, _ = run(cbx, d, r, plan, c, n_kv, group, rng, q=x["q"], kn=x["kn"], vn=x["vn"])
+    assert np.array_equal(got, want)
+
+
+def test_t3_prompts_without_a_list_of_tiles(small):  # noqa: F811
+    """The transformer's prompt rows, with the plan's tiles, none, and too few."""
+    torch, mod, s, dm, _ = small
+    x = torch.randn((70, N), device="cuda", generator=torch.Generator("cuda").manual_seed(2)) * 0.7
+    out = []
+    for tiles in ("listed", "none", "few"):
+        torch.manual_seed(1)
+        srv = Server(torch, mod, s, dm, 5, 0, torch.float32)
+        r = srv.rows(70, step=False, tiles=tiles == "listed")
+        srv.plan(r, n_new=[9, 0, 33, 27, 1])
+        if tiles == "few":
+            f = torch.zeros((1, 4), dtype=torch.int32, device="cuda")
+            r.tiles, r.n_tiles, r._tensors = f.data_ptr(), 1, r._tensors + (f,)
+        say("t3", tiles)
+        hid = torch.full((70, N), 7.0, device="cuda")
+        s.t3_kv(dm, srv.cache, srv.streams, r, hid, inputs=x)
+        torch.cuda.synchronize()
+        out.append(hid.cpu().numpy())
+    assert np.array_equal(out[0], out[1]) and np.array_equal(out[0], out[2])
+    assert np.isfinite(out[0]).all() and (out[0] != 7.0).all()

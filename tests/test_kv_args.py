@@ -222,3 +222,24 @@ def test_host_tensors_are_refused(lib):
         s.kv_attend(S.kv_attn(c, t, r, q, torch.empty_like(q)))
     with pytest.raises(ValueError, match="GPU 0"):
         s.t3_kv(mod.T3Model(), c, t, r, q, tokens=z(4))
+
+
+def test_prompts_without_a_list_of_tiles(lib):
+    """NULL tiles and n_tiles 0: found from row_start, as many as a list would
+    have (n_rows / tile_rows + n_streams) within a launch's limit; the Python view
+    leaves out a list that is too short, and no other."""
+    mod, so, handle = lib
+    a = attn(mod, dict(step=False, r=dict(tiles=None, n_tiles=0, tile_rows=0, n_rows=10),
+                       t=dict(n_streams=16384), c=dict(n_head=1024, n_pages=20),
+                       a=dict(n_head=1024, ld_q=65536, ld_kv=65536, ld_out=65536)))
+    assert 10 * 1024 + 16384 * 1024 > 0xffffff
+    refused(mod, so.cbx_kv_attend(handle, ctypes.byref(a), None), mod.CBX_ERR_UNSUPPORTED)
+    S, c, t, _ = view(mod)
+    q = z(100, 192, dt=torch.float32)
+    for n_tiles, tile_rows, kept in ((5, 64, True), (4, 64, False), (1, 64, False), (6, 64, True),
+                                     (4, 0, True)):
+        r = S.kv_rows(z(100), z(100), z(5), z(5), z(4), stream=z(100), tiles=z(n_tiles, 4),
+                      tile_rows=tile_rows)
+        got = S.kv_attn(c, t, r, q, torch.empty_like(q)).rows.contents
+        assert (got.n_tiles, bool(got.tiles)) == ((n_tiles, True) if kept else (0, False))
+        assert (r.n_tiles, bool(r.tiles)) == (n_tiles, True) and got.position == r.position
