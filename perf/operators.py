@@ -272,7 +272,7 @@ def prepare(case, seed):
         return s
     # the rows' map is built before the call, as once for all layers of a step; tiles only where
     # the call is to share prefixes, or walks prompts
-    tiles = _tiles_of(case, st["n"]) if case["shared"] or not step else 0
+    tiles = _tiles_of(dict(case, low=1), st["n"]) if case["shared"] or not step else 0
     n_rows = st["n"] if step else sum(n_new)
     rows = s["rows"] = _rows(st, case["form"], n_rows, tiles, _tile_rows(group))
     _plain_build(st, rows, s["n_new"], None)
