@@ -31,19 +31,19 @@ struct cbx_sampler {
     int32_t* static_redo = nullptr;
     // launches of at most this many row-steps run at full capacity
     int64_t latency_rows = cbx::kLatencyRows;
-    // the head's activation split (matrix-core projections), grown on demand
-    void* d_head = nullptr;
-    size_t head_bytes = 0;
-    // the T3 decode step's workspace, grown on demand
-    void* d_t3 = nullptr;
-    size_t t3_bytes = 0;
-    // whether a call that uses these was captured, and the buffers replaced
-    // since, which its graph still holds
+    // device memory grown on demand; captured: a graph may hold its address
+    struct Buffer {
+        void* p = nullptr;
+        size_t bytes = 0;
+        bool captured = false;
+    };
+    Buffer head;  // the head's activation split (matrix-core projections)
+    Buffer t3;    // the T3 decode step's workspace
+    // the captured ones of these that larger ones have replaced
     struct Kept {
         void* p;
         Kept* next;
     };
-    bool captured = false;
     Kept* kept = nullptr;
     // Pinned host memory that the single-row kernels read and write in place
     // (coherent: nothing of an earlier call stays in a cache): the row, the
@@ -126,8 +126,8 @@ void release(cbx_sampler* s) {
     (void)hipFree(s->d_probs);
     (void)hipFree(s->d_redo);
     (void)hipFree(s->d_redo_row);
-    (void)hipFree(s->d_head);
-    (void)hipFree(s->d_t3);
+    (void)hipFree(s->head.p);
+    (void)hipFree(s->t3.p);
     while (s->kept) {
         cbx_sampler::Kept* const k = s->kept;
         s->kept = k->next;
@@ -140,29 +140,29 @@ void release(cbx_sampler* s) {
 }
 
 // One of the handle's buffers for a call of `need` bytes on st: replaced by a
-// larger one where it is too small, but not while st is captured.
-int grow(const char* fn, cbx_sampler* s, void** p, size_t* bytes, size_t need, hipStream_t st) {
+// larger one where it is too small, but not while st is captured.  The old one
+// is freed, or kept for the graph where a call on it was captured.
+int grow(const char* fn, cbx_sampler* s, cbx_sampler::Buffer& b, size_t need, hipStream_t st) {
     hipStreamCaptureStatus c = hipStreamCaptureStatusNone;
     if (st && hipStreamIsCapturing(st, &c) != hipSuccess) (void)hipGetLastError();
     const bool capturing = c == hipStreamCaptureStatusActive;
-    if (need > *bytes) {
+    if (need > b.bytes) {
         if (capturing)
             return fail(CBX_ERR_UNSUPPORTED, "%s: the handle's buffer has %zu of %zu bytes: make a "
-                        "call of this size before one is captured", fn, *bytes, need);
-        if (s->captured && *p) {
-            cbx_sampler::Kept* const k = new (std::nothrow) cbx_sampler::Kept{*p, s->kept};
+                        "call of this size before one is captured", fn, b.bytes, need);
+        if (b.captured) {
+            cbx_sampler::Kept* const k = new (std::nothrow) cbx_sampler::Kept{b.p, s->kept};
             if (!k) return fail(CBX_ERR_NOMEM, "%s: out of host memory", fn);
             s->kept = k;
         } else {
             CBX_HIP(hipDeviceSynchronize());
-            CBX_HIP(hipFree(*p));
+            CBX_HIP(hipFree(b.p));
         }
-        *p = nullptr;
-        *bytes = 0;
-        CBX_HIP(hipMalloc(p, need));
-        *bytes = need;
+        b = cbx_sampler::Buffer();
+        CBX_HIP(hipMalloc(&b.p, need));
+        b.bytes = need;
     }
-    s->captured = s->captured || (capturing && need);
+    b.captured = b.captured || (capturing && need);
     return CBX_OK;
 }
 
@@ -536,11 +536,11 @@ int check_head(const char* fn, const cbx_head* h, int32_t n_rows, int32_t n_voca
 int run_head(cbx_sampler* s, const cbx_head* h, int32_t n_rows, int32_t n_vocab,
              int64_t ld_logits, hipStream_t st) {
     const size_t need = cbx::head_scratch_bytes(n_rows, h->hidden_uncond != nullptr, h->n_embd);
-    const int rc = grow("speech_head", s, &s->d_head, &s->head_bytes, need, st);
+    const int rc = grow("speech_head", s, s->head, need, st);
     if (rc != CBX_OK) return rc;
     CBX_HIP(cbx::launch_head(h->weights, h->wtype, h->bias, h->hidden, h->hidden_uncond,
                              h->ld_hidden, h->logits, h->logits_uncond, ld_logits, n_rows,
-                             n_vocab, h->n_embd, s->d_head, st));
+                             n_vocab, h->n_embd, s->head.p, st));
     return CBX_OK;
 }
 }  // namespace
@@ -779,11 +779,11 @@ int t3_run(const char* fn, cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows
     }
     DeviceGuard g(s->device);
     const size_t body = cbx::t3_workspace_bytes(n_rows, m->n_embd), need = body + kv_bytes;
-    const int rc = grow(fn, s, &s->d_t3, &s->t3_bytes, need, (hipStream_t)stream);
+    const int rc = grow(fn, s, s->t3, need, (hipStream_t)stream);
     if (rc != CBX_OK) return rc;
-    if (kv) a.workspace = static_cast<char*>(s->d_t3) + body;
+    if (kv) a.workspace = static_cast<char*>(s->t3.p) + body;
     CBX_HIP(cbx::launch_t3_step(*m, n_rows, tokens, inputs, positions, state, slots, n_slots,
-                                *cache, hidden, s->d_t3, (hipStream_t)stream, kv ? &a : nullptr));
+                                *cache, hidden, s->t3.p, (hipStream_t)stream, kv ? &a : nullptr));
     return CBX_OK;
 }
 }  // namespace
