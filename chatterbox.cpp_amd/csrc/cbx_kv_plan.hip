@@ -154,13 +154,14 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan(PlanArgs a) {
         return x;
     };
     if (a.release) {  // the pages given back, a wave copying a stream's at a time
-        int at = (int)(scan(n_back) - n_back);
+        int64_t at = scan(n_back) - n_back;  // lengths may claim any number of pages
         const int64_t all = total;
 #pragma unroll
         for (int u = 0; u < PER; ++u) {
             for (uint64_t left = __ballot(back[u] > 0); left; left &= left - 1) {
                 const int from = (int)__builtin_ctzll(left);
-                const int k = __shfl(back[u], from), to = n_free + __shfl(at, from);
+                const int k = __shfl(back[u], from);
+                const int64_t to = n_free + __shfl(at, from);
                 const int64_t src = (int64_t)((tid & ~63) + from) * PER + u;
                 for (int j = lane; j < k && to + j < a.s.n_pages; j += 64)
                     a.s.free_pages[to + j] = a.s.tables[src * a.s.max_pages + j];
