@@ -627,7 +627,7 @@ int check_kv(const char* fn, const cbx_kv_streams* t, const cbx_kv_rows* r, int3
             return fail(CBX_ERR_INVALID, "%s: tiles not 16-byte aligned, or without order", fn);
         const int64_t want = (int64_t)(r->tile_rows > 0 ? r->n_rows / r->tile_rows : 0) +
                              (r->stream ? t->n_streams : t->n_prefix);
-        if (r->tile_rows < 1 || r->n_tiles < (want > 1 ? want : 1))
+        if (r->tile_rows < 1 || r->tile_rows > 64 || r->n_tiles < (want > 1 ? want : 1))
             return fail(CBX_ERR_INVALID, "%s: %d tiles of %d rows, %lld wanted", fn, r->n_tiles,
                         r->tile_rows, (long long)want);
     }

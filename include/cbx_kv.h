@@ -75,7 +75,8 @@ typedef struct cbx_kv_rows {
     int32_t  n_rows;
     int32_t  n_tiles;    /* entries of tiles: at least n_rows / tile_rows + n_streams
                             (prompt form) or + n_prefix (step form)                  */
-    int32_t  tile_rows;  /* rows of a tile: cbx_kv_tile_rows(n_head, kv heads)       */
+    int32_t  tile_rows;  /* rows of a tile: cbx_kv_tile_rows(n_head, kv heads), 64
+                            at most                                                  */
     int32_t* stream;     /* [n_rows] or NULL                                         */
     int32_t* position;   /* [n_rows], a prefix's positions counted; -1: no row       */
     int32_t* slot;       /* [n_rows] page * page_size + place in the page; -1: none  */

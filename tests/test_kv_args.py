@@ -243,3 +243,14 @@ def test_prompts_without_a_list_of_tiles(lib):
         got = S.kv_attn(c, t, r, q, torch.empty_like(q)).rows.contents
         assert (got.n_tiles, bool(got.tiles)) == ((n_tiles, True) if kept else (0, False))
         assert (r.n_tiles, bool(r.tiles)) == (n_tiles, True) and got.position == r.position
+
+
+@pytest.mark.parametrize("step", [True, False])
+@pytest.mark.parametrize("tile_rows", [65, 2 ** 31 - 1])
+def test_tiles_of_more_than_64_rows_are_refused(lib, step, tile_rows):
+    """No attention takes them, and rows + tile_rows passes 32 bits in the plan."""
+    mod, so, handle = lib
+    t, r = streams(mod), rows(mod, step, tile_rows=tile_rows)
+    p = mod.KvPlan()
+    p.streams, p.rows, p.page_size = ctypes.pointer(t), ctypes.pointer(r), 16
+    refused(mod, so.cbx_kv_build(handle, ctypes.byref(p), None))
