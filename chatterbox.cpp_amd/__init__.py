@@ -837,7 +837,8 @@ class Sampler:
         """A cbx_kv_attn: q and out float32 [n_rows, 64 n_head], optional k and
         v [n_rows, 64 n_kv_head], each with unit stride along its rows (a
         view of wider rows will do).  Its workspace is allocated here unless
-        given (uint8): two calls that may run at once take a KvAttn each."""
+        given (uint8): two calls that may run at once take a KvAttn each.  A
+        graph that holds a call on it needs the KvAttn as long as it replays."""
         import torch
         dev = Sampler._one_call("kv_attn", streams, rows)
         rows = Sampler._with_tiles(streams, rows)
@@ -867,7 +868,8 @@ class Sampler:
             a.k, a.v, a.ld_kv = k.data_ptr(), v.data_ptr(), ld(k)
         need = load_library().cbx_kv_workspace_bytes(ctypes.byref(a))
         if workspace is None and need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            workspace = a._own_workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            a._made_on = torch.cuda.current_stream(dev).cuda_stream if dev.type == "cuda" else 0
         if workspace is not None:
             Sampler._check_kv("kv_attn", dev, workspace=(workspace, torch.uint8, (None,)))
             a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
@@ -880,6 +882,13 @@ class Sampler:
         self._on_device("kv_attend", attn._tensors[1])
         st = _stream_ptr() if stream is None else ctypes.c_void_p(stream)
         _check(self.lib.cbx_kv_attend(self.handle, ctypes.byref(attn), st))
+        # a workspace that the caller does not see may go back to torch's allocator
+        # while another stream than the one it was made on still uses it
+        ws = getattr(attn, "_own_workspace", None)
+        if ws is not None and (st.value or 0) != attn._made_on:
+            import torch
+            ws.record_stream(torch.cuda.ExternalStream(st.value, ws.device) if st.value
+                             else torch.cuda.default_stream(ws.device))
 
     def decode_step(self, logits, params, tokens, decode, **kw):
         """cbx_decode_step (head=...: cbx_head_decode_step) of one step."""

@@ -83,3 +83,36 @@ def test_t3_prompts_without_a_list_of_tiles(small):  # noqa: F811
         out.append(hid.cpu().numpy())
     assert np.array_equal(out[0], out[1]) and np.array_equal(out[0], out[2])
     assert np.isfinite(out[0]).all() and (out[0] != 7.0).all()
+
+
+# ------------------------------------------------------------------ streams
+
+
+def test_a_workspace_outlives_its_call_on_another_stream(cbx):  # noqa: F811
+    """A call put on a busy stream and its KvAttn dropped: torch does not hand the
+    workspace to the stream that it was made on until the call has ended."""
+    torch, mod, s = cbx
+    rng = np.random.default_rng(3)
+    pool = pool_of(rng, [1500, 900], 16)
+    d = Dev(torch, mod, pool)
+    d.plan(s, d.rows(False, 2400), n_new=[1500, 900])
+    c = caches(torch, rng, pool, 2, torch.float32)
+    store(torch, rng, pool, c, 0, [1500, 900])
+    r = d.rows(True, tiles=False)
+    plan = d.plan(s, r)
+    want, x = run(cbx, d, r, plan, c, 2, 1, rng)
+    side = torch.cuda.Stream()
+    out = torch.empty((2, 2 * D), device="cuda")
+    a = mod.Sampler.kv_attn(mod.Sampler.kv_cache(*c), d.streams, r, x["q"], out, k=x["kn"], v=x["vn"])
+    at, size = a.workspace, a.workspace_bytes
+    assert size
+    torch.cuda.synchronize()
+    say("another stream")
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+    s.kv_attend(a, stream=side.cuda_stream)
+    del a
+    other = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    assert at not in [t.data_ptr() for t in other]
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(), want)
