@@ -4,8 +4,11 @@ import numpy as np
 import pytest
 
 from oracle import cbx_kv_oracle as KV
-from test_gpu_kv import D, Dev, caches, cbx, run, say, store  # noqa: F401
-from test_gpu_kv_t3 import N, Server, small  # noqa: F401
+from oracle import cbx_t3_oracle as T3
+from test_gpu_kv import (D, Dev, caches, cbx, run, say, store, test_prompts_match_oracle as prompts_match,  # noqa: F401
+                         test_shared_prefix_matches_oracle as shared_matches,
+                         test_step_matches_oracle as step_matches)
+from test_gpu_kv_t3 import H, L_, N, TOL, V, Server, small  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +119,82 @@ def test_a_workspace_outlives_its_call_on_another_stream(cbx):  # noqa: F811
     assert at not in [t.data_ptr() for t in other]
     torch.cuda.synchronize()
     assert np.array_equal(out.cpu().numpy(), want)
+
+
+# ------------------------------------------------------------------ heads, pages, rows already stored
+
+
+@pytest.mark.parametrize("group", [16, 17, 40, 64])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_steps_of_many_heads_a_key_head(cbx, dtype, group):  # noqa: F811
+    """More pairs of a row than a wave holds: several workgroups a row, each with
+    the row's new key; prefixes' tiles of one to four rows."""
+    step_matches(cbx, [31, 0, 130, 64], dtype, 2, group, 16)
+    shared_matches(cbx, [40, 70], [(0, 40, 0), (0, 33, 100), (-1, 0, 20), (1, 70, 16), (1, 1, 7), (0, 2, 3)],
+                   dtype, 1, group, 16)
+
+
+@pytest.mark.parametrize("page", [128, 256])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_large_pages(cbx, dtype, page):  # noqa: F811
+    step_matches(cbx, [127, 0, 128, 700, 255, 256], dtype, 2, 1, page)
+    step_matches(cbx, [300, 1], dtype, 2, 4, page)
+    shared_matches(cbx, [300], [(0, 300, 0), (0, 255, 130), (0, 257, 255), (-1, 0, 256)], dtype, 2, 1, page)
+    prompts_match(cbx, [200], [(0, 200, 100, 200), (0, 129, 0, 127), (-1, 0, 256, 3)], dtype, 2, 1, page)
+
+
+@pytest.mark.parametrize("n_kv,group", [(2, 1), (1, 4)])
+@pytest.mark.parametrize("n", [3, 90], ids=["few", "many"])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_rows_already_stored(cbx, dtype, n, n_kv, group):  # noqa: F811
+    """Calls without new keys and values: the cache holds them."""
+    torch, mod, s = cbx
+    rng = np.random.default_rng(n)
+    had = [50] + [(5 * i) % 61 for i in range(n)]
+    say("stored", dtype, n, n_kv, group)
+    new = [0] + [1 + (7 * i) % 50 for i in range(n)]
+    pool = pool_of(rng, [a + b for a, b in zip(had, new)], 16, 1, [-1] + [0] * n,
+                   [0] + [(50, 33, 0)[i % 3] for i in range(n)])
+    d = Dev(torch, mod, pool)
+    d.plan(s, d.rows(False, sum(had)), n_new=had)
+    c = caches(torch, rng, pool, n_kv, getattr(torch, dtype))
+    store(torch, rng, pool, c, 0, had)
+    T = mod.Sampler.kv_tile_rows(n_kv * group, n_kv)
+    for step in (False, True):
+        r = d.rows(step, sum(new), tile_rows=T)
+        plan = d.plan(s, r, n_new=[0] + [1] * n if step else new)
+        run(cbx, d, r, plan, c, n_kv, group, rng, sd=2.0)
+        run(cbx, d, r, plan, c, n_kv, group, rng, sd=2.0, new=False)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_t3_steps_of_whole_rows(small, dtype):  # noqa: F811
+    """As many streams as rows are not cut for: each row goes from its one
+    workgroup straight into the next product's parts.  The tolerance is
+    test_gpu_kv_t3.py's."""
+    torch, mod, s, dm, rm = small
+    n, half = 256, dtype == "float16"
+    say("t3 whole rows", dtype)
+    rng = np.random.default_rng(12)
+    srv = Server(torch, mod, s, dm, n, 0, getattr(torch, dtype), n_pages=3 * n)
+    oracles = [T3.new_cache(n, L_, H, 64)]
+    if half:
+        oracles.append(tuple(c.astype(np.float16) for c in T3.new_cache(n, L_, H, 64)))
+    own = np.array([1 + (7 * i) % 30 for i in range(n)])
+    x = (rng.standard_normal((own.sum(), N)) * 0.7).astype(np.float32)
+    srv.prompt(x, own.tolist())
+    for i, f in enumerate(np.cumsum(own) - own):
+        for c in oracles:
+            T3.prefill(rm, x[f:f + own[i]], *c, i, 0)
+    moved = 0.0
+    for turn in range(3):
+        tokens, state = rng.integers(0, V, n), [1 if i % 9 == turn else 0 for i in range(n)]
+        active = np.array(state) == 0
+        got = srv.step(tokens, state, False)
+        want = [T3.step(rm, tokens, own.copy(), *c, active=active) for c in oracles]
+        if half:
+            moved = max(moved, np.abs(want[1] - want[0])[active].max())
+        err = np.abs(got - want[-1]) - TOL * np.abs(want[-1])
+        assert err[active].max() <= TOL + 2 * moved, (turn, err[active].max(), moved)
+        assert np.all(got[~active] == 0.0)
+        own[active] += 1
