@@ -4,14 +4,15 @@
 //
 // A row's positions [0, n) are its prefix's [0, plen), in the prefix's pages,
 // then its own, in its own pages from their first place on.  The softmax is
-// taken in one pass, e^x as 2^(x log2 e): over any set of keys, with a whole
-// number r >= max x log2 e, (r, s, o) = (r, sum w, sum w v), w = 2^(x log2 e - r),
-// and two sets join as
+// taken in one pass, e^x as 2^y, y = x log2 e (the scale that queries are
+// multiplied by holds log2 e): over any set of keys, with a whole number r near
+// the largest y, (r, s, o) = (r, sum w, sum w v), w = 2^(y - r), and two sets join as
 //   r = max(r1, r2), s = s1 2^(r1 - r) + s2 2^(r2 - r), o alike; out = o / s,
 // so keys may be cut anywhere: over lanes, waves, workgroups, and into a
 // prefix's part computed once for many rows and each row's own.  r whole: every
-// rescaling is by a power of two, and x log2 e - r one fused operation whose r
-// is the same for all keys of a set, so no rounding of the reference remains.
+// rescaling is by a power of two.  y is one value for a key wherever it is met and
+// y - r is exact where it matters (the two are near), so r leaves no rounding of its
+// own, at any size of the scores.
 //
 //  * kv_rows: the step form, one row a stream, on the vector units: what
 //    bounds it is reading each stream's keys and values.
@@ -46,8 +47,6 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float rescale(float from, float to) {
     return from == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(__fsub_rn(from, to));
 }
-// The reference of scores up to x (c2: the scores' unit in powers of two).
-__device__ __forceinline__ float reference(float x, float c2) { return __builtin_ceilf(__fmul_rn(x, c2)); }
 
 struct KvArgs {
     const void* kc;  // this layer's pages: [page][n_kv][position][64]
@@ -70,7 +69,7 @@ struct KvArgs {
     int64_t ld_kv;
     int32_t n_head, group;  // query heads, of them per key head
     uint32_t over_group;    // x / group = x * over_group >> 16 for x < 128
-    float scale;
+    float scale;            // times log2 e
     AttnOut o;
     // parts of rows cut over workgroups, [part][n_rows][n_head]: (m, s) and
     // o[64]; the rows' own parts first, then their prefixes' (n_own 0: none,
@@ -288,7 +287,7 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
                 }
 #pragma unroll
                 for (int u = 0; u < kU; ++u) bm = fmaxf(bm, x[u]);
-                const float nr = fmaxf(m[g], reference(bm, kLog2e));
+                const float nr = fmaxf(m[g], __builtin_ceilf(bm));
                 if (__ballot(nr > m[g])) {
                     const float f = rescale(m[g], nr);
                     s[g] = __fmul_rn(s[g], f);
@@ -297,10 +296,10 @@ __device__ __forceinline__ void rows_of(const KvArgs& a, uint32_t block, int par
                     m[g] = nr;
                 }
                 // a key that is not there, or -inf while none is larger, has weight 0
-                const float off = m[g] == -INFINITY ? 0.0f : -m[g];
+                const float off = m[g] == -INFINITY ? 0.0f : m[g];
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const float e = __builtin_amdgcn_exp2f(__fmaf_rn(x[u], kLog2e, off));
+                    const float e = __builtin_amdgcn_exp2f(__fsub_rn(x[u], off));
                     s[g] = __fadd_rn(s[g], e);
 #pragma unroll
                     for (int d = 0; d < DPL; ++d) o[g][d] = __fmaf_rn(C::at(vv[u], d), e, o[g][d]);
@@ -888,10 +887,10 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         if (F16) odd4 = (float)odd8[0] + (float)odd8[1];
         if (odd4 != odd4) odd[slot] = 1;
     };
-    // q, scaled: dimensions 32 ks + 8 g .. of pair c, in parts; c2: a score as the
-    // matrix cores give it to powers of two
+    // q, scaled: dimensions 32 ks + 8 g .. of pair c, in parts; c2: the power of two
+    // that a score as the matrix cores give it is short of
     u4 qp[2][P::kQ];
-    float c2 = kLog2e;
+    float c2 = 1.0f;
     {
         const float* const qr = a.q + rc * a.ld_q + (real ? h : 0) * kDim;
         float x[2][8], mx = 0.0f;
@@ -909,9 +908,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         float sc = 1.0f;
         if (F16) {
             mx = max_column(mx);
-            float inv;
-            split_scale(mx, sc, inv);
-            c2 = __fmul_rn(kLog2e, inv);
+            split_scale(mx, sc, c2);
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
@@ -929,8 +926,9 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
     f4 o[4];
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) o[dt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    // the exponents' offset and the exponent that moves the reference, kept with it
-    float ref = -INFINITY, off = kUp, bar = -INFINITY;
+    // the reference, negated (kUp below the largest exponent when it was chosen), and
+    // how far over it an exponent moves it (-inf: no key yet)
+    float off = 0.0f, bar = -INFINITY;
     f4 sum = f4{0.0f, 0.0f, 0.0f, 0.0f};  // the first of it
     int last = lim, least = real ? lim : INT32_MAX;
     const auto over = [&](auto x) {  // lanes at a distance of x
@@ -986,8 +984,8 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
                 for (int i = 0; i < 4; ++i)
                     if (!(see >> (16 * kt + i) & 1)) x[kt][i] = -INFINITY;
         }
-        // exponents by the pair's reference (by 0 before it has one); a larger one
-        // than kSlack over it moves the reference up
+        // exponents by the pair's reference (0 before it has one); a larger one than
+        // kUp + kSlack over it moves the reference up
         float top = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -999,13 +997,11 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         top = max_column(top);
         const bool move = top > bar;
         if (__ballot(move)) {
-            const float by = move ? __builtin_ceilf(__fsub_rn(top, kUp)) : 0.0f;
-            const float f = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by);
-            ref = !move ? ref : ref == -INFINITY ? by : __fadd_rn(ref, by);
-            if (move) {
-                off = __fsub_rn(kUp, ref);
-                bar = kUp + kSlack;
-            }
+            const float to = move ? __fsub_rn(off, __fsub_rn(__builtin_ceilf(top), kUp)) : off;
+            const float by = __fsub_rn(off, to);  // as far as it moves, once rounded
+            const float f = bar == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by);
+            off = to;
+            if (move) bar = kUp + kSlack;
             sum[0] = __fmul_rn(sum[0], f);
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt)
@@ -1124,7 +1120,7 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         *reinterpret_cast<f4*>(os + ce * kPad + 16 * i + 4 * ge) = o[i];
     }
     if (ge == 0) {
-        join_m[we][ce] = ref;
+        join_m[we][ce] = bar == -INFINITY ? -INFINITY : -off;
         join_s[we][ce] = sum[0];
     }
     __syncthreads();
@@ -1133,11 +1129,10 @@ __device__ __forceinline__ void tiles_of(const KvArgs& a, uint32_t block, uint32
         const int ri = __shfl(row_end >= 0 ? row_end : a.n_rows, i), hi = __shfl(h_end, i);
         if (FORM == kPrefix || (FORM == kOneRow && a.n_own > 0)) {
             if (ri >= a.n_rows) return;
-            constexpr float kDown = F16 ? 1.0f / 16384.0f : 1.0f;
             const int part = (FORM == kPrefix ? a.n_own : 0) + cut;
             const int64_t to = ((int64_t)part * a.n_rows + ri) * a.n_head + hi;
-            if (ce == 0) a.part_ms[to] = float2{pm, __fmul_rn(ps, kDown)};
-            *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * ce) = po * kDown;
+            if (ce == 0) a.part_ms[to] = float2{pm, ps};
+            *reinterpret_cast<f4*>(a.part_o + to * kDim + 4 * ce) = po;
         } else {
             const float over = ps == 0.0f ? 0.0f : __fdiv_rn(1.0f, ps);
             attn_store4(a.o, a.n_rows, ri, hi, ce, po * over);
@@ -1370,7 +1365,7 @@ hipError_t launch_kv_attend(const cbx_kv_attn& c, uint32_t* parts, float* inv, h
     a.n_head = c.n_head;
     a.group = c.n_head / p.n_head;
     a.over_group = 65536 / a.group + 1;
-    a.scale = c.scale;
+    a.scale = c.scale * kLog2e;
     a.o = AttnOut{c.out, c.ld_out, parts, inv, c.n_head};
     const uint64_t n = (uint64_t)(cut.own + cut.shared) * r.n_rows * c.n_head;
     a.part_ms = static_cast<float2*>(c.workspace);

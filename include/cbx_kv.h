@@ -133,10 +133,12 @@ int cbx_kv_build(cbx_sampler* s, const cbx_kv_plan* p, void* stream);
  * a row with a position whose page is not one of the pool's does not see those
  * positions; a row that sees none gives zeros.  Keys and values that a row does
  * not see never reach it, whatever they hold.  A query or a seen key that is
- * not finite leaves its own row's outputs undefined, no other's.
+ * not finite leaves its own row's outputs undefined, no other's; so does a score
+ * of 2^127 or more, or a seen value of 2^80.
  * Sums and softmax statistics are fp32.  Products are fp32's, or on the 16-bit
  * matrix cores of values cut into parts: fp32 caches' into three bf16 parts
- * (each product to 2^-21 of itself); fp16 caches' queries and weights into two
+ * (each product to 2^-21 of itself, of values that are 0 or 2^-100 and more in
+ * magnitude); fp16 caches' queries and weights into two
  * fp16 parts (to 2^-22 and 2^-20 of themselves, or 2^-38 of the row's largest).
  * n_rows * n_head, with tiles + n_tiles * cache->n_head (prompts without a list:
  * as many as it would have), is at most 2^24 - 1,

@@ -10,7 +10,7 @@ value, the third below 2^-15):
  * a score: three products of nine left out, below 2 * 2^-22 + 2^-30, 8 u of it;
    six added, the smallest first: two additions that count, 4 u, the others' sums
    are below 2^-6 of it: 12 * 2^-6 < 1 u.                          13 u
- * the exponent x log2 e rounded once at its own size, log2 e once:  2 u
+ * the scale times log2 e rounded once, the query by it once:        2 u
    so a weight is off by 15 u S, an output by twice that of A = sum p |v|.
  * w v: products left out 8 u; six additions of two keys' 12 u; the weights' sum
    three additions, 6 u; 2^x to 1 ulp in numerator and denominator, 4 u; the joins
@@ -19,7 +19,7 @@ value, the third below 2^-15):
    |out - ref| <= A u (30 S + 36).
 fp16 caches, keys and values as they are, queries in two parts (to 2^-22, 4 u) and
 weights in two (cut off, to 2^-20, 16 u, in the sum too):
- * a score: 4 u, two additions 4 u; the exponent 2 u:                10 u
+ * a score: 4 u, two additions 4 u; the scale and the query 2 u:     10 u
  * w v: 2 * 16 u; two additions each of products and weights 8 u; 2^x 4 u; joins 4 u;
    the division 2 u.                                                 50 u
    |out - ref| <= A u (20 S + 50).
@@ -100,7 +100,7 @@ def product(a, b, dtype, left_out, acc=np.float32(0.0)):
 
 def model(q, k, v, dtype, scores_without=-1, values_without=-1, scale=0.125):
     """One query [m][64] each against two keys and values [2][m][64]."""
-    s = (q * np.float32(scale)).astype(np.float32)
+    s = (q * np.float32(scale * np.log2(np.e))).astype(np.float32)
     # to [2^14, 2^15), and the weights to 2^14: their lower parts lose nothing
     up = np.exp2(14 - np.floor(np.log2(np.abs(s).max(-1)))).astype(np.float32) if dtype == "float16" \
         else np.ones(len(q), np.float32)
@@ -110,7 +110,7 @@ def model(q, k, v, dtype, scores_without=-1, values_without=-1, scale=0.125):
         a, b = (np.take_along_axis(t, d, -1)[:, 0] for t in (k[i], s))
         x.append(product(a, b * up, dtype, scores_without))
     x = np.stack(x)
-    e = (x.astype(np.float64) / up * np.log2(np.e)).astype(np.float32)
+    e = x / up
     w = np.exp2(e.astype(np.float64) - np.ceil(e.max(0))).astype(np.float32)
     w = w * np.float32(2 ** 14 if dtype == "float16" else 1)
     o = np.zeros(v.shape[1:], np.float32)

@@ -5,9 +5,10 @@ import pytest
 
 from oracle import cbx_kv_oracle as KV
 from oracle import cbx_t3_oracle as T3
-from test_gpu_kv import (D, Dev, caches, cbx, run, say, store, test_prompts_match_oracle as prompts_match,  # noqa: F401
-                         test_shared_prefix_matches_oracle as shared_matches,
-                         test_step_matches_oracle as step_matches)
+from test_gpu_kv import D, Dev, bound, caches, cbx, run, say, store  # noqa: F401
+from test_gpu_kv import test_prompts_match_oracle as prompts_match
+from test_gpu_kv import test_shared_prefix_matches_oracle as shared_matches
+from test_gpu_kv import test_step_matches_oracle as step_matches
 from test_gpu_kv_t3 import H, L_, N, TOL, V, Server, small  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -198,3 +199,121 @@ def test_t3_steps_of_whole_rows(small, dtype):  # noqa: F811
         assert err[active].max() <= TOL + 2 * moved, (turn, err[active].max(), moved)
         assert np.all(got[~active] == 0.0)
         own[active] += 1
+
+
+# ------------------------------------------------------------------ large scores
+
+
+@pytest.mark.parametrize("form", ["step", "shared", "prompt"])
+@pytest.mark.parametrize("size", [1e6, 1e10, 1e20, -1e10, -1e30])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_large_scores(cbx, dtype, group, size, form):  # noqa: F811
+    """Finite scores of any size: the j-th key from the end has size (1 + j / 64),
+    so one key of each row is larger than all others by size / 64 at least and the
+    output is its value: a weight of 1, or a power of two, and the division, each
+    rounded once or twice (8 u; fp16 parts of a weight that is no power of two cut
+    off at 2^-20 in the sum and the product alike, 32 u)."""
+    torch, mod, s = cbx
+    rng = np.random.default_rng(4)
+    say("large", dtype, group, size, form)
+    n_kv, n, plen = 2, 5, 20
+    own = [0, 3, 17, 40, 63]
+    n0 = 1 if form == "shared" else 0
+    had = [plen] * n0 + [x - (x > plen) * plen if n0 else x for x in own]
+    pool = pool_of(rng, had, 16, n0, [-1] * n0 + [n0 - 1] * n, [0] * n0 + [plen] * n)
+    d = Dev(torch, mod, pool)
+    d.plan(s, d.rows(False, sum(had) + 1), n_new=had)
+    c = caches(torch, rng, pool, n_kv, getattr(torch, dtype))
+    store(torch, rng, pool, c, 0, had)
+    T = mod.Sampler.kv_tile_rows(n_kv * group, n_kv)
+    new = [0] * n0 + [1] * n
+    r = d.rows(form != "prompt", sum(new), tiles=form != "step", tile_rows=T)
+    plan = d.plan(s, r, n_new=new)
+    rows = [i for i in range(r.n_rows) if plan["position"][i] >= 0]
+    # keys: 1 + j / 64 (exact in either type) in dimension 0 alone, j shuffled over
+    # the positions that a row sees
+    kc, vc = (t[0].float().cpu().numpy() for t in c)
+    kc[:] = 0.0
+    kn = np.zeros((r.n_rows, n_kv, D), np.float32)
+    vn = rng.standard_normal((r.n_rows, n_kv, D)).astype(np.float32)
+    if dtype == "float16":
+        vn = vn.astype(np.float16).astype(np.float32)
+    want = np.zeros((r.n_rows, n_kv, D))
+    shared = rng.permutation(plen) if n0 else []
+    for x in range(plen if n0 else 0):
+        kc[pool.tables[0, x // 16], :, x % 16, 0] = 1 + shared[x] / 64
+    for i in rows:
+        st, pos = (i if form != "prompt" else plan["stream"][i]), int(plan["position"][i])
+        mine = pos + 1 - (plen if n0 else 0)
+        j = list(shared) + list(rng.permutation(mine) + len(shared))
+        at = KV.keys_of(pool, st, pos)
+        for x in range(len(shared), pos):
+            kc[at[x][0], :, at[x][1], 0] = 1 + j[x] / 64
+        kn[i, :, 0] = 1 + j[pos] / 64
+        best = int(np.argmax(j) if size > 0 else np.argmin(j))
+        want[i] = vn[i] if best == pos else vc[at[best][0], :, at[best][1]]
+    for t, x in zip(c, (kc, vc)):
+        t[0].copy_(torch.from_numpy(x))
+    q = np.zeros((r.n_rows, n_kv * group, D), np.float32)
+    q[..., 0] = size * 8
+    out = torch.empty((r.n_rows, n_kv * group * D), device="cuda")
+    t = lambda a: torch.from_numpy(a.reshape(r.n_rows, -1)).cuda()  # noqa: E731
+    s.kv_attend(mod.Sampler.kv_attn(mod.Sampler.kv_cache(*c), d.streams, r, t(q), out, k=t(kn), v=t(vn)))
+    got = out.cpu().numpy().reshape(r.n_rows, n_kv, group, D)[rows]
+    want = want[rows][:, :, None]
+    assert np.abs(got - want).max() <= 40 * 2.0 ** -24 * np.abs(want).max(), np.abs(got - want).max((1, 2, 3))
+
+
+@pytest.mark.parametrize("form", ["step", "few", "many"])
+@pytest.mark.parametrize("size", [1.0, 1e6, 3e7, 1e9, 1e10, 1e20, -3e7, -1e10, -1e30])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("group", [1, 4])
+def test_large_equal_scores(cbx, dtype, group, size, form):  # noqa: F811
+    """Keys of two kinds, all scores of a kind the same to the bit, wherever they
+    are met: the output is the mean of the larger kind's values (at size 1 the
+    softmax of both), within the bound of n equal scores; the larger kind first,
+    last, or in turn."""
+    torch, mod, s = cbx
+    rng = np.random.default_rng(6)
+    say("equal", dtype, group, size, form)
+    n_kv, lens = 2, [0, 5, 40, 100, 333] + [70] * (60 if form == "many" else 0)
+    pool = pool_of(rng, lens, 16)
+    d = Dev(torch, mod, pool)
+    d.plan(s, d.rows(False, sum(lens)), n_new=lens)
+    c = caches(torch, rng, pool, n_kv, getattr(torch, dtype))
+    store(torch, rng, pool, c, 0, lens)
+    T = mod.Sampler.kv_tile_rows(n_kv * group, n_kv)
+    r = d.rows(form == "step", len(lens), tiles=form != "step", tile_rows=T)
+    plan = d.plan(s, r, n_new=[1] * len(lens))
+    vn = rng.standard_normal((len(lens), n_kv, D)).astype(getattr(np, dtype)).astype(np.float32)
+    t = lambda a: torch.from_numpy(a.reshape(len(lens), -1)).cuda()  # noqa: E731
+    q = np.zeros((len(lens), n_kv * group, D), np.float32)
+    q[..., 0] = size * 8
+    for order in ("first", "last", "turn"):
+        kc, vc = (x[0].float().cpu().numpy() for x in c)
+        kc[:] = 0.0
+        kn = np.zeros_like(vn)
+        want, mass, n_keys = np.zeros((len(lens), n_kv, D)), np.zeros((len(lens), n_kv, D)), []
+        for i, L in enumerate(lens):
+            big = {"first": np.arange(L + 1) <= L // 2, "last": np.arange(L + 1) >= L // 2,
+                   "turn": np.arange(L + 1) % 2 == 0}[order]
+            at = KV.keys_of(pool, i, L)
+            vs = np.zeros((L + 1, n_kv, D))
+            for x in range(L + 1):
+                if x < L:
+                    kc[at[x][0], :, at[x][1], 0] = 1 + big[x] / 64
+                    vs[x] = vc[at[x][0], :, at[x][1]]
+            kn[i, :, 0], vs[L] = 1 + big[L] / 64, vn[i]
+            p = np.exp(size * (1 + big / 64) - (size * (1 + big / 64)).max())
+            p = (p / p.sum())[:, None, None]
+            want[i], mass[i] = (p * vs).sum(0), (p * np.abs(vs)).sum(0)
+            n_keys.append(L + 1)
+        c[0][0].copy_(torch.from_numpy(kc))
+        out = torch.empty((len(lens), n_kv * group * D), device="cuda")
+        s.kv_attend(mod.Sampler.kv_attn(mod.Sampler.kv_cache(*c), d.streams, r, t(q), out, k=t(kn), v=t(vn)))
+        got = out.cpu().numpy().reshape(len(lens), n_kv, group, D)
+        near = 2.0 if size == 1.0 else 0.0
+        lim = bound(np.full((len(lens), n_kv), near), mass, np.array(n_keys))[:, :, None]
+        worst = (np.abs(got - want[:, :, None]) / lim).max((1, 2, 3))
+        assert worst.max() <= 1.0, (order, worst[:5])
