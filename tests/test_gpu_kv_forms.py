@@ -317,3 +317,106 @@ def test_large_equal_scores(cbx, dtype, group, size, form):  # noqa: F811
         lim = bound(np.full((len(lens), n_kv), near), mass, np.array(n_keys))[:, :, None]
         worst = (np.abs(got - want[:, :, None]) / lim).max((1, 2, 3))
         assert worst.max() <= 1.0, (order, worst[:5])
+
+
+# ------------------------------------------------------------------ queries and keys that are not finite
+
+
+@pytest.mark.parametrize("what", ["query", "key"])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("form", ["few", "many", "shared"])
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_queries_and_keys_that_are_not_finite_stay(cbx, dtype, group, form, bad, what):  # noqa: F811
+    """One query, or one key, reaches its own row, or the rows that see it, alone:
+    all others are bit for bit the same."""
+    torch, mod, s = cbx
+    n_kv, H = 2, 2 * group
+    n = [40, 21] if form == "few" else [90] * 60 if form == "many" else [1] * 9
+    say("not finite", what, bad, form, group, dtype)
+    out = []
+    for plant in (False, True):
+        rng = np.random.default_rng(5)
+        n0 = 1 if form == "shared" else 0
+        lens = [40] * n0 + [4 * n0] * len(n)
+        share = [(40, 37, 12, 9)[i % 4] for i in range(len(n))]
+        pool = KV.Pool(n0 + len(n), 8, 16, 500, n_prefix=n0, parent=[-1] * n0 + [n0 - 1] * len(n),
+                       prefix_len=[0] * n0 + share)
+        d = Dev(torch, mod, pool)
+        c = caches(torch, rng, pool, n_kv, getattr(torch, dtype))
+        if n0:
+            d.plan(s, d.rows(False, sum(lens)), n_new=lens)
+            store(torch, rng, pool, c, 0, lens)
+        r = d.rows(bool(n0), sum(n), tile_rows=64 // group)
+        d.plan(s, r, n_new=[0] * n0 + n)
+        x = torch.from_numpy(rng.standard_normal((r.n_rows, (H + 2 * n_kv) * D)).astype(np.float32)).cuda()
+        if n0:
+            row, pos = 1 + 2, 12  # the third stream's query; the prefix's key 12, that two of four see
+            hit = [row] if what == "query" else [1 + i for i in range(len(n)) if share[i] > pos]
+            if plant and what == "key":
+                c[0][0, int(pool.tables[0, 0]), 0, pos, 7] = bad
+        else:
+            row = n[0] + 9        # the second stream's tenth position
+            hit = [row] if what == "query" else list(range(row, n[0] + n[1]))
+            if plant and what == "key":
+                x[row, H * D + 7] = bad
+        if plant and what == "query":
+            x[row, 7] = bad
+        o = torch.empty((r.n_rows, H * D), device="cuda")
+        q, k, v = x[:, :H * D], x[:, H * D:(H + n_kv) * D], x[:, (H + n_kv) * D:]
+        s.kv_attend(mod.Sampler.kv_attn(mod.Sampler.kv_cache(*c), d.streams, r, q, o, k=k, v=v))
+        torch.cuda.synchronize()
+        out.append(o.cpu().numpy().reshape(-1, H, D))
+    same = np.ones(out[0].shape[:2], bool)
+    same[hit, :1 if what == "query" else group] = False
+    assert np.isfinite(out[0]).all() and np.array_equal(out[0][same], out[1][same])
+
+
+# ------------------------------------------------------------------ offsets past 32 bits
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_offsets_past_32_bits(cbx, dtype):  # noqa: F811
+    """A pool of more than 2^32 values a layer, its second layer's last pages used."""
+    torch, mod, s = cbx
+    n_kv, page, used = 4, 256, 12
+    n_pages = (1 << 32) // (n_kv * page * D) + 300
+    say("past 32 bits", dtype)
+    assert n_pages * n_kv * page < 2 ** 32 - 1 and n_pages * page < 2 ** 31
+    k, v = (torch.empty((2, n_pages, n_kv, page, D), dtype=getattr(torch, dtype), device="cuda")
+            for _ in range(2))
+    rng = np.random.default_rng(1)
+    lens = [300, 20, 511]
+    for form in ("step", "shared", "prompt"):
+        n0 = 1 if form == "shared" else 0
+        pool = KV.Pool(3, 4, page, n_pages, n_prefix=n0, parent=[-1] + [n0 - 1] * 2,
+                       prefix_len=[0, 300, 270] if n0 else [0] * 3)
+        d = Dev(torch, mod, pool)  # the stack's top: the last pages
+        d.plan(s, d.rows(False, sum(lens)), n_new=lens)
+        r = d.rows(form != "prompt", 90, tiles=form != "step")
+        plan = d.plan(s, r, n_new=[0 if n0 else 1, 1, 1] if form != "prompt" else [40, 30, 20])
+        first = n_pages - used
+        host = [rng.standard_normal((used, n_kv, page, D)).astype(dtype) for _ in range(2)]
+        for t, x in zip((k, v), host):
+            t[1, first:] = torch.from_numpy(x).cuda()
+        x = rng.standard_normal((r.n_rows, 3 * n_kv * D)).astype(np.float32)
+        rows = torch.from_numpy(x).cuda()
+        q, kn, vn = rows.split(n_kv * D, dim=1)
+        out = torch.empty((r.n_rows, n_kv * D), device="cuda")
+        s.kv_attend(mod.Sampler.kv_attn(mod.Sampler.kv_cache(k, v), d.streams, r, q, out, layer=1, k=kn, v=vn))
+        torch.cuda.synchronize()
+        for row, sl in enumerate(plan["slot"]):
+            if sl >= 0:
+                for h, t in zip(host, (kn, vn)):
+                    h[sl // page - first, :, sl % page] = t[row].reshape(n_kv, D).to(k.dtype).cpu().numpy()
+        for t, h in zip((k, v), host):
+            assert np.array_equal(t[1, first:].cpu().numpy(), h)
+        small_pool = KV.Pool(3, 4, page, used, n_prefix=n0, parent=pool.parent, prefix_len=pool.prefix_len)
+        small_pool.tables[:] = pool.tables - first
+        stream = plan.get("stream", np.arange(3))
+        want, size, mass, n_keys = KV.attend(small_pool, *[h.astype(np.float32) for h in host], stream,
+                                             plan["position"], q.cpu().numpy(), 0.125)
+        lim = bound(size, mass, n_keys).reshape(want.shape)
+        assert (np.abs(out.cpu().numpy() - want) <= lim).all(), form
+    del k, v
+    torch.cuda.empty_cache()

@@ -46,3 +46,5 @@ def test_more_pages_given_back_than_32_bits_count(cbx):
     want[guard:guard + had] = -3
     want[guard + had:guard + n_pages] = np.arange(n_pages - had)
     assert np.array_equal(buf.cpu().numpy(), want)
+    del tables, plan
+    torch.cuda.empty_cache()
