@@ -146,7 +146,7 @@ struct Chunk<_Float16> {
 
 // One part of one row's keys, for G of its key head's query heads, by W waves
 // (4: a workgroup; 1: the workgroup's waves take a head each, with no barrier).
-// Bound by the bytes: 64 rows of 129 to 383 fp32 keys 28.7 us, 4.7 TB/s.
+// Bound by the bytes: 64 rows of 129 to 383 fp32 keys 29 us, 4.65 TB/s; fp16 14.8.
 // LPK lanes to a key, 16 bytes of it each, kU keys per lane in flight; the page
 // ids of 64 pages are held by the wave's lanes, and handed over by an exchange.
 // Each lane group keeps a running (m, s, o) of its keys, joined over the groups
@@ -567,11 +567,11 @@ struct Walk {
 // parts stored; or one row's heads of a key head against the row's keys, cut
 // likewise (where many query heads share a key head: the step form on the
 // vector units then spends its time on products).
-// Prompts of 4 x 4096 rows take fp32 965 us (142 TFLOP/s of the formula's, 850
-// of the parts'), fp16 530 (260, 585): the vector units' instructions (half the
-// time fp32, 60 % fp16) and the matrix cores' (43 %, 29 %) together.  64 prompts
-// of 129 to 383 rows fp32 129 us, 3.1 TB/s; 8 of 301 to 1501 fp16 behind 377 keys
-// 124.  What made them faster: loads that stand behind the choice of their
+// Prompts of 4 x 4096 rows take fp32 965 to 990 us (139 to 142 TFLOP/s of the
+// formula's, six times as many of the parts' without the weights' sums), fp16 525
+// (262, twice as many): the vector units' instructions (half the time fp32, 60 %
+// fp16) and the matrix cores' (43 %, 30 %) together.  64 prompts of 129 to 383 rows
+// fp32 130 us, 3.1 TB/s; 8 of 301 to 1501 fp16 behind 377 keys 125.  What made them faster: loads that stand behind the choice of their
 // addresses (fp16 8 %), the longest tiles first (7 %), four workgroups a CU for
 // fp16 (8 %), nothing kept over the loop that its end can find again (up to
 // 7 %).  What did not: fewer instructions for a stage's addresses, all of K's
@@ -1198,7 +1198,13 @@ __global__ __launch_bounds__(256, 3) void kv_shared(KvArgs a, uint32_t tile_bloc
 // ------------------------------------------------------------------ launches
 
 // How a call's keys are cut: parts of a row's own (0: whole rows, stored by
-// the workgroup itself) and of a prefix.
+// the workgroup itself) and of a prefix.  Lengths are the device's: the host knows
+// the tables' capacity alone, and cuts for rows as long as that.  Parts that a
+// shorter row does not need end at once, but are launched, and its one part goes
+// through the workspace and the join: us, tables of 416 / 8196 positions, 64 rows
+// of 129 to 383 fp32 keys 29 / 43 (2048: 33, 32768: 87), 63 of them 34 / 42, fp16
+// 64 14.8 / 31, 64 of up to 300 behind a prefix of 377 18 / 32; 256 fp16 rows of 64
+// to 4001 with four query heads a key head 76 (3968) / 84.
 struct Cut {
     int own, shared, min_part;
 };

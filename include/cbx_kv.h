@@ -55,7 +55,9 @@ typedef struct cbx_kv_streams {
     int32_t  n_streams;        /* 1 .. 16384                                         */
     int32_t  n_prefix;         /* 0 .. n_streams                                     */
     int32_t  max_pages;        /* pages a stream holds at most; max_pages * page_size
-                                  below 2^30                                         */
+                                  below 2^30.  The step form's attention cuts rows
+                                  by this capacity, not by their lengths: where it is
+                                  many times the rows' it costs time                 */
     int32_t  n_pages;          /* the pool's                                         */
     int32_t* tables;           /* [n_streams][max_pages] page ids, in position order */
     int32_t* len;              /* [n_streams] positions stored in its own pages      */

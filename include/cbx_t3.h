@@ -124,10 +124,12 @@ int cbx_t3_prefill(cbx_sampler* s, const cbx_t3_model* m, int32_t n_rows,
  * rows; so does a row whose position is outside [0, n_pos) or whose token is
  * outside [0, n_speech_vocab): the keys stored for it are a zero input's.
  * tile_rows is cbx_kv_tile_rows(n_head, n_head).  Sums and products as in
- * cbx_t3_step; the handle holds the workspace, so calls on one handle are
- * ordered on one stream.  A call may be captured once a call of its size has run
- * (CBX_ERR_UNSUPPORTED before); larger calls later leave the graph's workspace
- * to it until the handle is destroyed.  Replaces eval_step and eval_prompt
+ * cbx_t3_step, but for the attention's products of prompts and of prefixes that
+ * come with tiles: those are cbx_kv_attend's, on the 16-bit matrix cores.  The
+ * handle holds the workspace, so calls on one handle are ordered on one stream.
+ * A call may be captured once a call of its size has run (CBX_ERR_UNSUPPORTED
+ * before); a larger call later leaves the graph's workspace to it until the
+ * handle is destroyed.  Replaces eval_step and eval_prompt
  * (main.cpp:643-710) up to ln_f. */
 int cbx_t3_kv(cbx_sampler* s, const cbx_t3_model* m, const cbx_kv_cache* cache,
               const cbx_kv_streams* streams, const cbx_kv_rows* rows, const int32_t* tokens,
